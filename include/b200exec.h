@@ -209,6 +209,161 @@ int rt_fusion_report(const OpNode* nodes, int n_nodes, int* flags);
 int rt_matmul_noalloc(const float* a, const float* b, const float* bias, float* c,
                       int M, int N, int K, int trans_b, float alpha, void* stream);
 
+/* ---- serving: paged key/value cache ------------------------------------- */
+/* No counterpart in the reference, whose text generation re-plans and re-runs
+ * the whole prefix for every token (run_gpt2.py:92-113).  These calls are what
+ * a decoder runs beside its planned graph instead: they store the keys and
+ * values of new tokens in the pages of a cache, attend over them, read them
+ * back, and verify drafted tokens.
+ *
+ * All of them need rt_init, enqueue on the caller's `stream` (a cudaStream_t
+ * of that device; NULL = legacy default stream) and return without waiting;
+ * they allocate nothing and may be captured into a CUDA graph.  Arguments are
+ * checked on the host before anything is enqueued.  What only the device can
+ * see (slots, page numbers, lengths, offsets) is bounds-checked by the
+ * kernels: an entry out of range is treated as absent and reported as
+ * RT_ERR_OUT_OF_RANGE by the next rt_check_stream / rt_synchronize. */
+enum RtDtype { RT_F32 = 0, RT_BF16 = 1, RT_F8E4M3 = 2, RT_I8 = 3 };
+
+/* One layer's cache, owned by the caller.  Element d of head h in slot s of
+ * page p is k[p*stride[0] + s*stride[1] + h*stride[2] + d] (v alike); the
+ * features are contiguous, k, v and the strides (in bytes) multiples of 16,
+ * head_dim a multiple of 16 up to 128.  RT_F32 / RT_BF16 hold the values;
+ * RT_F8E4M3 / RT_I8 hold codes, and the value is code * scale with one scale
+ * per (page, slot, head) at k_scale[p*scale_stride[0] + s*scale_stride[1] +
+ * h*scale_stride[2]] (NULL otherwise). */
+typedef struct RtKvCache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t stride[3];
+    int64_t scale_stride[3];
+    int dtype;
+    int n_pages;
+    int page_size;
+    int n_heads;
+    int head_dim;
+} RtKvCache;
+
+/* Stores n_tokens rows of k and v (dtype RT_F32 / RT_BF16; element (token,
+ * head, d) at token*stride[0] + head*stride[1] + d) into the cache: token i
+ * goes to slot slots[i] = page * page_size + position in the page; a negative
+ * slot skips the token.  Two tokens of one call must not share a slot.  For 8
+ * bits, with a = max |x| over the token's head and M = 127 (I8) or 448
+ * (F8E4M3), in fp32 with every step rounded: scale = a * (1/M), code = x *
+ * ((1/a) * M) to the nearest code, ties to even; a < 2^-100 stores zeros with
+ * scale 0, a non-finite value in the head stores zeros with scale NaN (the
+ * head reads back as NaN). */
+typedef struct RtKvWrite {
+    RtKvCache cache;
+    const void* k;
+    const void* v;
+    int64_t k_stride[2];
+    int64_t v_stride[2];
+    const int64_t* slots;
+    int dtype;
+    int n_tokens;
+} RtKvWrite;
+int rt_kv_write(const RtKvWrite* w, void* stream);
+
+/* Reads cached positions back as dense rows: row cu[b] + i of k_out / v_out
+ * (dtype RT_F32 / RT_BF16, element (row, head, d) at row*stride[0] +
+ * head*stride[1] + d) is position start[b] + i of sequence b, i < cu[b+1] -
+ * cu[b] (start NULL: 0).  Position j of sequence b lies in page
+ * page_table[b*table_stride + j / page_size].  n_rows rows are written: those
+ * from cu[n_seqs] on, and those whose position has no page, are zero. */
+typedef struct RtKvRead {
+    RtKvCache cache;
+    void* k_out;
+    void* v_out;
+    int64_t k_stride[2];
+    int64_t v_stride[2];
+    const int* page_table;
+    int64_t table_stride;
+    const int* start;
+    const int* cu;
+    int dtype;
+    int n_seqs;
+    int table_width;
+    int n_rows;
+} RtKvRead;
+int rt_kv_read(const RtKvRead* r, void* stream);
+
+/* Attention of new tokens over the cache.  Sequence b brings the tokens
+ * cu_new[b] .. cu_new[b+1]-1 of q (element (token, head, d) at token*stride[0]
+ * + head*stride[1] + d; out alike) and has kv_lens[b] cached positions, the
+ * new tokens' own (written before this call) included.  The new token i of n
+ * stands at position P = kv_lens[b] - n + i and sees positions j <= P (causal)
+ * or all of them, and with window > 0 only j > P - window.  out = softmax(q.k
+ * * scale) v with query head h reading cache head h / (n_q_heads / n_heads);
+ * lse (may be NULL, [tokens][n_q_heads]) = log of the softmax's sum.  A token
+ * that sees nothing gets out = 0, lse = -inf.  Positions that no token of the
+ * call sees are never read into the result, whatever they hold.
+ * max_new / max_kv: the host's bounds on the per-sequence counts; they choose
+ * how the work is split, not what is computed.  `ws` holds
+ * rt_paged_attention_workspace(p) bytes of device memory, 16-byte aligned, used by
+ * this call alone until it has run. */
+typedef struct RtPagedAttention {
+    RtKvCache cache;
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t q_stride[2];
+    int64_t out_stride[2];
+    const int* page_table;
+    int64_t table_stride;
+    const int* kv_lens;
+    const int* cu_new;
+    float scale;
+    int dtype;
+    int n_seqs;
+    int table_width;
+    int n_q_heads;
+    int total_new;
+    int max_new;
+    int max_kv;
+    int causal;
+    int window;
+} RtPagedAttention;
+size_t rt_paged_attention_workspace(const RtPagedAttention* p);
+int rt_paged_attention(const RtPagedAttention* p, void* ws, size_t ws_bytes, void* stream);
+
+/* Verification of drafted tokens (speculative sampling).  Row (b, i) of the
+ * target's probabilities (dtype RT_F32 / RT_BF16, vocabulary contiguous, at
+ * b*target_stride[0] + i*target_stride[1]) is the distribution of the token at
+ * draft position i, row n_drafts the one after all drafts; draft holds the
+ * draft's rows (NULL: every draft was proposed with probability 1).  Draft i
+ * is accepted when accept_u[b*n_drafts + i] * draft(x_i) < target(x_i) and all
+ * before it were; draft_lens[b] (NULL: n_drafts) of them exist.  The next
+ * token is sampled from max(target - draft, 0) of the first refused row (from
+ * target if nothing is left of it), or from the target's row after the last
+ * draft: weights w become integers floor(min(w, 1) * 2^40) (negative or NaN:
+ * 0), and the token is the lowest one whose running sum exceeds
+ * floor(floor(u * 2^24) * total / 2^24), u = sample_u[b] in [0, 1).
+ * tokens[b*(n_drafts+1) ..]: the accepted drafts, the sampled token (-1: the
+ * row has no mass), then -1; accepted[b]: how many drafts were accepted. */
+typedef struct RtVerifyDraft {
+    const void* target;
+    const void* draft;
+    int64_t target_stride[2];
+    int64_t draft_stride[2];
+    const int* draft_tokens;
+    const int* draft_lens;
+    const float* accept_u;
+    const float* sample_u;
+    int* tokens;
+    int* accepted;
+    int dtype;
+    int n_seqs;
+    int n_drafts;
+    int vocab;
+} RtVerifyDraft;
+int rt_verify_draft(const RtVerifyDraft* v, void* stream);
+
+/* Waits for `stream` and returns what its kernels reported. */
+int rt_check_stream(void* stream);
+
 /* ---- errors ------------------------------------------------------------- */
 /* No counterpart in the reference (which never waits on the device).  Runs
  * one kernel whose single bounded mbarrier wait is never satisfied, with a

@@ -218,6 +218,28 @@ Status launch_norm(const OpNode& n, cudaStream_t st, int* launches);
 Status launch_reduce(const OpNode& n, cudaStream_t st, int* launches);
 Status launch_layout(const OpNode& n, cudaStream_t st, int* launches);
 
+// ---- serving calls (serving.cu checks arguments, these launch) --------------
+Status launch_kv_write(const RtKvWrite& w, cudaStream_t st);
+Status launch_kv_read(const RtKvRead& r, cudaStream_t st);
+size_t paged_attention_workspace(const RtPagedAttention& p);
+Status launch_paged_attention(const RtPagedAttention& p, void* ws, cudaStream_t st);
+Status launch_verify_draft(const RtVerifyDraft& v, cudaStream_t st);
+inline int dtype_bytes(int t) { return t == RT_F32 ? 4 : t == RT_BF16 ? 2 : 1; }
+
+// What the entry points outside runtime.cu need of its state.
+bool runtime_ready();
+int runtime_device();
+int report(const Status& s);   // records a failure for rt_last_error and returns its code
+// Device memory of the initialised device, `bytes` of it where the allocation is ours.
+Status check_device_pointer(const void* p, size_t bytes, const char* what);
+// After a synchronise: what a kernel left in the error word, as a status.
+Status kernel_status();
+int* kernel_error_flag();
+// Codes of the error word: 0x400.. an index read from device memory was out
+// of range, everything else an abandoned wait.
+constexpr int KERR_SLOT = 0x401, KERR_PAGE = 0x402, KERR_LENGTH = 0x403, KERR_TOKEN = 0x404;
+constexpr int KERR_RANGE_FIRST = 0x400, KERR_RANGE_LAST = 0x4ff;
+
 inline int grid_for(int64_t work_items, int threads, int per_sm = 8) {
     int64_t blocks = (work_items + threads - 1) / threads;
     int64_t cap = (int64_t)g_num_sms * per_sm;

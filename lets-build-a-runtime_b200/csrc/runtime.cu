@@ -636,6 +636,32 @@ int take_kernel_error() {
     return v;
 }
 
+Status kernel_status() {
+    const int k = take_kernel_error();
+    if (!k) return Status::ok();
+    if (k >= KERR_RANGE_FIRST && k <= KERR_RANGE_LAST) {
+        const char* what = k == KERR_SLOT     ? "a cache slot"
+                           : k == KERR_PAGE   ? "a page number"
+                           : k == KERR_LENGTH ? "a sequence length or offset"
+                                              : "a drafted token";
+        return Status::err(RT_ERR_OUT_OF_RANGE, std::string(what) + " in device memory was out of range");
+    }
+    return Status::err(RT_ERR_KERNEL_TIMEOUT, "a kernel abandoned a bounded wait, code " + std::to_string(k));
+}
+
+bool runtime_ready() { return S().initialized; }
+int runtime_device() { return S().device; }
+int report(const Status& s) {
+    std::lock_guard<std::recursive_mutex> g(M());
+    return fail(s);
+}
+Status check_device_pointer(const void* p, size_t bytes, const char* what) {
+    std::lock_guard<std::recursive_mutex> g(M());
+    Status s = check_buffer(p, bytes, 0, what);
+    if (!s.good() && s.msg.rfind("node 0: ", 0) == 0) s.msg.erase(0, 8);
+    return s;
+}
+
 // A wait that nothing will ever complete: one thread waits on an mbarrier
 // that no thread arrives on, through the same bounded wait the tensor-core
 // kernels use.  After limit_ns it records ERR_PROBE in the error word and
@@ -852,8 +878,7 @@ int rt_execute(const OpNode* nodes, int n, int flags) {
     if (!(flags & RT_FLAG_ASYNC)) {
         cudaError_t e = cudaStreamSynchronize(st);
         if (e != cudaSuccess) return fail(RT_ERR_CUDA, std::string("execute: ") + cudaGetErrorString(e));
-        if (int k = take_kernel_error())
-            return fail(RT_ERR_KERNEL_TIMEOUT, "a kernel abandoned a bounded wait, code " + std::to_string(k));
+        if (Status ks = kernel_status(); !ks.good()) return fail(ks);
     }
     return RT_OK;
 }
@@ -882,8 +907,7 @@ int rt_execute_io(const OpNode* nodes, int n, const RtCopy* h2d, int n_in, const
     }
     cudaError_t e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return fail(RT_ERR_CUDA, std::string("execute_io: ") + cudaGetErrorString(e));
-    if (int k = take_kernel_error())
-        return fail(RT_ERR_KERNEL_TIMEOUT, "a kernel abandoned a bounded wait, code " + std::to_string(k));
+    if (Status ks = kernel_status(); !ks.good()) return fail(ks);
     return RT_OK;
 }
 
@@ -929,8 +953,7 @@ int rt_execute_chunks(const RtChunk* chunks, int n_chunks) {
     }
     cudaEventDestroy(ready);
     if (e != cudaSuccess) return fail(RT_ERR_CUDA, std::string("execute_chunks: ") + cudaGetErrorString(e));
-    if (int k = take_kernel_error())
-        return fail(RT_ERR_KERNEL_TIMEOUT, "a kernel abandoned a bounded wait, code " + std::to_string(k));
+    if (Status ks = kernel_status(); !ks.good()) return fail(ks);
     return RT_OK;
 }
 
@@ -1012,8 +1035,7 @@ int rt_synchronize(void) {
     RT_NEED_INIT;
     cudaError_t e = cudaStreamSynchronize(S().stream);
     if (e != cudaSuccess) return fail(RT_ERR_CUDA, cudaGetErrorString(e));
-    if (int k = take_kernel_error())
-        return fail(RT_ERR_KERNEL_TIMEOUT, "a kernel abandoned a bounded wait, code " + std::to_string(k));
+    if (Status ks = kernel_status(); !ks.good()) return fail(ks);
     return RT_OK;
 }
 
@@ -1071,8 +1093,7 @@ int rt_check_wait_timeout(unsigned long long limit_ns) {
     if (e != cudaSuccess) return fail(RT_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
     e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return fail(RT_ERR_CUDA, std::string("wait probe: ") + cudaGetErrorString(e));
-    if (int k = take_kernel_error())
-        return fail(RT_ERR_KERNEL_TIMEOUT, "a kernel abandoned a bounded wait, code " + std::to_string(k));
+    if (Status ks = kernel_status(); !ks.good()) return fail(ks);
     return RT_OK;
 }
 
