@@ -1,10 +1,25 @@
 // k_paged_attention.cu -- attention of new tokens over a paged cache: which
 // kernel takes a call.
+//
+// More than 16 rows (new tokens x query heads of a cache head) fill a tensor
+// core tile of 128 well enough to beat reading the cache once per 16 rows;
+// head dims other than 64 and 128 have no such tiles and take the few-rows
+// kernel whatever their rows.
 #include "paged.h"
 
 namespace rt {
+namespace {
 
-size_t paged_attention_workspace(const RtPagedAttention& p) { return paged_few_workspace(p); }
+bool use_tiles(const RtPagedAttention& p) {
+    const int64_t rows = (int64_t)(p.max_new < p.total_new ? p.max_new : p.total_new) * (p.n_q_heads / p.cache.n_heads);
+    return rows > 16 && paged_tiles_takes(p);
+}
+
+}  // namespace
+
+size_t paged_attention_workspace(const RtPagedAttention& p) {
+    return use_tiles(p) ? paged_tiles_workspace(p) : paged_few_workspace(p);
+}
 
 Status launch_paged_attention(const RtPagedAttention& a, void* ws, cudaStream_t st) {
     PagedArgs p{};
@@ -14,7 +29,7 @@ Status launch_paged_attention(const RtPagedAttention& a, void* ws, cudaStream_t 
     p.page_shift = -1;
     for (int i = 0; i < 31; i++)
         if (a.cache.page_size == 1 << i) p.page_shift = i;
-    return launch_paged_few(p, ws, st);
+    return use_tiles(a) ? launch_paged_tiles(p, ws, st) : launch_paged_few(p, ws, st);
 }
 
 }  // namespace rt

@@ -29,7 +29,6 @@
 //   the rest: tf32 products, q, weights and an fp32 cache's K and V as hi + lo
 //     (22 bits); bf16 K and V are exact in tf32.
 // Scores, maxima, weight sums and outputs are fp32.
-#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -620,59 +619,13 @@ __global__ void __launch_bounds__(FT) paged_few_kernel(const __grid_constant__ P
                 part[e] = sum;
                 if (d == 0) part[R * DP + r] = m, part[R * DP + R + r] = ls;
             } else if (d < D) {
-                const int rr = row0 + r, tok = rr / p.group, hq = cur.h * p.group + rr % p.group;
-                const int64_t row = s.first + tok;
-                const float x = ls == 0.0f ? 0.0f : sum / ls;
-                const int64_t at = row * p.a.out_stride[0] + hq * p.a.out_stride[1] + d;
-                if (act_bf16) static_cast<__nv_bfloat16*>(p.a.out)[at] = __float2bfloat16_rn(x);
-                else static_cast<float*>(p.a.out)[at] = x;
-                if (p.a.lse && d == 0)
-                    p.a.lse[row * p.a.n_q_heads + hq] = ls == 0.0f ? -INFINITY : (m + log2f(ls)) * 0.6931471805599453f;
+                paged_store(p, s, cur.h, row0 + r, d, ls == 0.0f ? 0.0f : sum / ls);
+                if (d == 0) paged_store_lse(p, s, cur.h, row0 + r, m, ls);
             }
         }
         __syncthreads();
         u += p.whole ? 1 : seg;
         cur.next_item<R, FKT>(p);
-    }
-}
-
-// Adds up the items that fell into several blocks: block c looks at the
-// boundary between blocks c and c + 1 of the main kernel.
-template <int DP, int R, int KT>
-__global__ void __launch_bounds__(FT) paged_join_kernel(const __grid_constant__ PagedArgs p, int blocks) {
-    __shared__ int sched[FT / 32 + 2];
-    PagedCursor cur;
-    int u, per, total;
-    const bool some = paged_schedule<FT, R, KT>(p, blockIdx.x + 1, blocks, sched, cur, u, per, total);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!some || cur.i == 0) return;
-    const int first = u - cur.i, c0 = blockIdx.x;
-    if (first < c0 * per) return;                          // an earlier boundary lies in this item
-    const int c1 = (first + cur.t.count - 1) / per;
-    constexpr int SLOT = R * DP + 2 * R;
-    const PagedSeq& s = cur.s;
-    const int row0 = cur.qt * R, rows = min(R, s.n * p.group - row0);
-    for (int e = threadIdx.x; e < rows * DP; e += FT) {
-        const int r = e / DP, d = e % DP;
-        float m = -INFINITY;
-        for (int c = c0; c <= c1; c++) m = fmaxf(m, p.part[(int64_t)(2 * c + (c == c0)) * SLOT + R * DP + r]);
-        float sum = 0.0f, ls = 0.0f;
-        if (m != -INFINITY)
-            for (int c = c0; c <= c1; c++) {
-                const float* part = p.part + (int64_t)(2 * c + (c == c0)) * SLOT;
-                const float f = exp2_fast(part[R * DP + r] - m);
-                if (f == 0.0f) continue;
-                sum += part[e] * f;
-                ls += part[R * DP + R + r] * f;
-            }
-        if (d >= p.a.cache.head_dim) continue;
-        const int rr = row0 + r, tok = rr / p.group, hq = cur.h * p.group + rr % p.group;
-        const int64_t row = s.first + tok;
-        const float x = ls == 0.0f ? 0.0f : sum / ls;
-        const int64_t at = row * p.a.out_stride[0] + hq * p.a.out_stride[1] + d;
-        if (p.a.dtype == RT_BF16) static_cast<__nv_bfloat16*>(p.a.out)[at] = __float2bfloat16_rn(x);
-        else static_cast<float*>(p.a.out)[at] = x;
-        if (p.a.lse && d == 0) p.a.lse[row * p.a.n_q_heads + hq] = ls == 0.0f ? -INFINITY : (m + log2f(ls)) * 0.6931471805599453f;
     }
 }
 
@@ -716,17 +669,7 @@ Status few_as(PagedArgs& p, void* ws, cudaStream_t st) {
     paged_few_kernel<CT, F32ACT, DP, R><<<blocks, FT, F::SMEM, st>>>(p);
     RT_LAUNCH_CHECK();
     if (p.whole || blocks == 1) return Status::ok();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks - 1);
-    cfg.blockDim = dim3(FT);
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // starts early, waits for the main kernel itself
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_join_kernel<DP, R, FKT>, p, blocks));
-    return Status::ok();
+    return launch_paged_join<DP, R, FKT>(p, blocks, st);
 }
 
 // Rows of a tile: 8 when that covers a call's rows and the hi / lo parts need

@@ -13,6 +13,8 @@
 // it starts, slot 2c from the others); the join kernel adds them in block
 // order, so results do not depend on timing.
 #pragma once
+#include <cuda_bf16.h>
+
 #include "rt_internal.h"
 
 namespace rt {
@@ -196,11 +198,87 @@ __device__ __forceinline__ float exp2_fast(float x) {   // 2^x; 2^-inf = 0
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// Feature d of row `row` (of the sequence's rows under cache head h), and the
+// row's log-sum-exp from its maximum (log2 units) and weight sum.
+__device__ __forceinline__ int64_t paged_out_at(const PagedArgs& p, const PagedSeq& s, int h, int row) {
+    return (int64_t)(s.first + row / p.group) * p.a.out_stride[0] + (h * p.group + row % p.group) * p.a.out_stride[1];
+}
+__device__ __forceinline__ void paged_store(const PagedArgs& p, const PagedSeq& s, int h, int row, int d, float x) {
+    const int64_t at = paged_out_at(p, s, h, row) + d;
+    if (p.a.dtype == RT_BF16) static_cast<__nv_bfloat16*>(p.a.out)[at] = __float2bfloat16_rn(x);
+    else static_cast<float*>(p.a.out)[at] = x;
+}
+__device__ __forceinline__ void paged_store_lse(const PagedArgs& p, const PagedSeq& s, int h, int row, float m, float l) {
+    if (p.a.lse)
+        p.a.lse[(int64_t)(s.first + row / p.group) * p.a.n_q_heads + h * p.group + row % p.group] =
+            l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// Adds up the items that fell into several blocks: block (c, y) looks at the
+// boundary between blocks c and c + 1 of the main kernel, and takes rows
+// 16 y .. of the item.  Started early (its own schedule overlaps the main
+// kernel's tail), it waits for the main kernel before it reads.
+constexpr int JOIN_ROWS = 16, JOIN_THREADS = 128;
+template <int DP, int R, int KT>
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_constant__ PagedArgs p, int blocks) {
+    __shared__ int sched[JOIN_THREADS / 32 + 2];
+    PagedCursor cur;
+    int u, per, total;
+    const bool some = paged_schedule<JOIN_THREADS, R, KT>(p, blockIdx.x + 1, blocks, sched, cur, u, per, total);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!some || cur.i == 0) return;
+    const int first = u - cur.i, c0 = blockIdx.x;
+    if (first < c0 * per) return;                          // an earlier boundary lies in this item
+    const int c1 = (first + cur.t.count - 1) / per;
+    constexpr int SLOT = R * DP + 2 * R;
+    const PagedSeq& s = cur.s;
+    const int row0 = cur.qt * R, rows = min(R, s.n * p.group - row0);
+    for (int e = threadIdx.x; e < JOIN_ROWS * DP / 4; e += JOIN_THREADS) {
+        const int r = blockIdx.y * JOIN_ROWS + e / (DP / 4), d = e % (DP / 4) * 4;
+        if (r >= rows) return;
+        float m = -INFINITY;
+        for (int c = c0; c <= c1; c++) m = fmaxf(m, p.part[(int64_t)(2 * c + (c == c0)) * SLOT + R * DP + r]);
+        float sum[4] = {0, 0, 0, 0}, ls = 0.0f;
+        if (m != -INFINITY)
+#pragma unroll 4
+            for (int c = c0; c <= c1; c++) {
+                const float* part = p.part + (int64_t)(2 * c + (c == c0)) * SLOT;
+                const float f = exp2_fast(part[R * DP + r] - m);
+                if (f == 0.0f) continue;
+                const float4 x = *reinterpret_cast<const float4*>(part + r * DP + d);
+                sum[0] += x.x * f; sum[1] += x.y * f; sum[2] += x.z * f; sum[3] += x.w * f;
+                ls += part[R * DP + R + r] * f;
+            }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (d + j < p.a.cache.head_dim) paged_store(p, s, cur.h, row0 + r, d + j, ls == 0.0f ? 0.0f : sum[j] / ls);
+        if (d == 0) paged_store_lse(p, s, cur.h, row0 + r, m, ls);
+    }
+}
+template <int DP, int R, int KT>
+Status launch_paged_join(const PagedArgs& p, int blocks, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks - 1, (R + JOIN_ROWS - 1) / JOIN_ROWS);
+    cfg.blockDim = dim3(JOIN_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_join_kernel<DP, R, KT>, p, blocks));
+    return Status::ok();
+}
 #endif
 
 // One launch (and the join, when items can be split): k_paged_few.cu for
 // tiles of 8 or 16 rows on the warp-level matrix instructions.
 size_t paged_few_workspace(const RtPagedAttention& p);
 Status launch_paged_few(PagedArgs& p, void* ws, cudaStream_t st);
+// k_paged_tiles.cu for tiles of 128 rows on the tensor cores (tcgen05).
+bool paged_tiles_takes(const RtPagedAttention& p);
+size_t paged_tiles_workspace(const RtPagedAttention& p);
+Status launch_paged_tiles(PagedArgs& p, void* ws, cudaStream_t st);
 
 }  // namespace rt

@@ -213,6 +213,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// 8 consecutive 32-bit columns of this warp's 32 lanes, from registers.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Generic-proxy shared-memory writes made visible to the async proxy (MMA / TMA).
 __device__ __forceinline__ void fence_proxy_async_smem() {
@@ -233,6 +239,48 @@ __device__ __forceinline__ uint64_t smem_desc(const void* base, uint32_t sbo_byt
     d |= (uint64_t)(layout & 7) << 61;                  // swizzle mode
     return d;
 }
+
+// Descriptors kept as 32-bit halves.  The upper half is a constant for
+// 128-byte-swizzled operands (groups of 8 rows 1024 bytes apart), the lower
+// one holds the start address and the leading byte offset; an operand's tiles
+// and K steps differ by a constant in the lower half, which the forms below
+// add inside the instruction group, so that an unrolled series of MMAs keeps
+// two registers alive instead of a descriptor per step.
+constexpr uint32_t DESC_HI_SW128 = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(const void* base, uint32_t lbo_bytes = 16) {
+    return ((smem_u32(base) >> 4) & 0x3FFFu) | (lbo_bytes >> 4) << 16;
+}
+// kind::f16 MMA, A and B in shared memory, at desc + OA / OB (units of 16 bytes).
+template <uint32_t OA, uint32_t OB>
+__device__ __forceinline__ void mma_f16_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "add.u32 x, %1, %5;\n\t"
+        "add.u32 y, %2, %6;\n\t"
+        "mov.b64 a, {x, %7};\n\t"
+        "mov.b64 b, {y, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(OA), "n"(OB), "r"(DESC_HI_SW128)
+        : "memory");
+}
+// The same with A in TMEM at column a + CA (8 columns per K step of 16).
+template <uint32_t CA, uint32_t OB>
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "add.u32 x, %1, %5;\n\t"
+        "add.u32 y, %2, %6;\n\t"
+        "mov.b64 b, {y, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(CA), "n"(OB), "r"(DESC_HI_SW128)
+        : "memory");
+}
+// Instruction descriptor flag: B's rows run along its non-contracted dimension,
+// one row per contracted element ("MN-major"; the leading byte offset then
+// goes from one 128-byte column block to the next).
+constexpr uint32_t IDESC_B_MN = 1u << 16;
 
 // Instruction descriptor for kind::tf32 with fp32 accumulation, both
 // operands K-major, tile M x N.
