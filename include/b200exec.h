@@ -224,6 +224,11 @@ int rt_matmul_noalloc(const float* a, const float* b, const float* bias, float* 
  * kernels: an entry out of range is treated as absent and reported as
  * RT_ERR_OUT_OF_RANGE by the next rt_check_stream / rt_synchronize. */
 enum RtDtype { RT_F32 = 0, RT_BF16 = 1, RT_F8E4M3 = 2, RT_I8 = 3 };
+/* The caller has established that every pointer of the call is memory of the
+ * library's device and spans what the sizes and strides say (a tensor library
+ * knows): the library then skips its own query of each pointer, which costs
+ * more than the launch for the smallest calls. */
+#define RT_POINTERS_CHECKED 1
 
 /* One layer's cache, owned by the caller.  Element d of head h in slot s of
  * page p is k[p*stride[0] + s*stride[1] + h*stride[2] + d] (v alike); the
@@ -244,6 +249,7 @@ typedef struct RtKvCache {
     int page_size;
     int n_heads;
     int head_dim;
+    int flags;   /* RT_POINTERS_CHECKED, for all pointers of the call */
 } RtKvCache;
 
 /* Stores n_tokens rows of k and v (dtype RT_F32 / RT_BF16; element (token,
@@ -358,6 +364,7 @@ typedef struct RtVerifyDraft {
     int n_seqs;
     int n_drafts;
     int vocab;
+    int flags;   /* RT_POINTERS_CHECKED */
 } RtVerifyDraft;
 int rt_verify_draft(const RtVerifyDraft* v, void* stream);
 

@@ -1,4 +1,5 @@
-"""Build libb200exec.so in-tree with nvcc for sm_100a.
+"""Build libb200exec.so in-tree with nvcc for sm_100a, and b200paged, the
+CPython module that calls it with torch tensors (host code, g++).
 
     python lets-build-a-runtime_b200/build.py        # or build() from Python
 
@@ -13,6 +14,7 @@ import concurrent.futures as cf
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -20,6 +22,7 @@ REPO = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "lib" / "libb200exec.so"
+EXT = PKG / "lib" / ("b200paged" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
@@ -68,7 +71,31 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}")
+    build_ext(verbose)
     return LIB
+
+
+def build_ext(verbose: bool = False) -> Path:
+    src = CSRC / "paged_ext.cpp"
+    header = REPO / "include" / "b200exec.h"
+    if EXT.exists() and all(EXT.stat().st_mtime >= p.stat().st_mtime for p in (src, header)):
+        return EXT
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(REPO / "include"), "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
+           str(src), "-o", str(EXT), "-L", str(LIB.parent), "-lb200exec", "-L", str(root / "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{r.stderr}")
+    return EXT
 
 
 if __name__ == "__main__":

@@ -27,6 +27,12 @@ struct DeviceGuard {
     }
 };
 
+thread_local bool t_checked = false;   // the call's pointers need no query
+Status check_pointer(const void* p, size_t bytes, const char* what) {
+    if (t_checked) return p || !bytes ? Status::ok() : Status::err(RT_ERR_NULL_POINTER, std::string(what) + " is NULL");
+    return check_device_pointer(p, bytes, what);
+}
+
 #define CHECK(expr)                \
     do {                           \
         Status _s = (expr);        \
@@ -59,8 +65,8 @@ Status check_cache(const RtKvCache& c) {
     // kernels keep a row's place in units of 16 bytes in 32 bits
     if (elems * e / 16 >= 0xffffffffll) return Status::err(RT_ERR_UNSUPPORTED, "cache: k and v must span less than 64 GiB each");
     if ((int64_t)c.n_pages * c.page_size > 0x7fffffffll) return Status::err(RT_ERR_UNSUPPORTED, "cache: more than 2^31 - 1 slots");
-    CHECK(check_device_pointer(c.k, (size_t)elems * e, "cache k"));
-    CHECK(check_device_pointer(c.v, (size_t)elems * e, "cache v"));
+    CHECK(check_pointer(c.k, (size_t)elems * e, "cache k"));
+    CHECK(check_pointer(c.v, (size_t)elems * e, "cache v"));
     if (e == 1) {
         int64_t s = 0;
         for (int i = 0; i < 3; i++)
@@ -68,8 +74,8 @@ Status check_cache(const RtKvCache& c) {
         s = span(c.n_pages, c.scale_stride[0], c.page_size, c.scale_stride[1], (c.n_heads - 1) * c.scale_stride[2] + 1);
         if (s > 0x7fffffffll) return Status::err(RT_ERR_UNSUPPORTED, "cache: scales span more than 2^31 - 1 elements");
         if (!c.k_scale || !c.v_scale) return Status::err(RT_ERR_NULL_POINTER, "cache: an 8-bit cache needs k_scale and v_scale");
-        CHECK(check_device_pointer(c.k_scale, (size_t)s * 4, "cache k_scale"));
-        CHECK(check_device_pointer(c.v_scale, (size_t)s * 4, "cache v_scale"));
+        CHECK(check_pointer(c.k_scale, (size_t)s * 4, "cache k_scale"));
+        CHECK(check_pointer(c.v_scale, (size_t)s * 4, "cache v_scale"));
     }
     return Status::ok();
 }
@@ -78,28 +84,30 @@ Status check_rows(const void* p, const int64_t st[2], int64_t rows, int heads, i
     if (st[0] < 0 || st[1] < 0) return bad(std::string(what) + ": negative stride");
     const int e = dtype_bytes(dtype);
     if (reinterpret_cast<uintptr_t>(p) % e) return bad(std::string(what) + ": not aligned to its element size");
-    return check_device_pointer(p, (size_t)span(rows, st[0], heads, st[1], dim) * e, what);
+    return check_pointer(p, (size_t)span(rows, st[0], heads, st[1], dim) * e, what);
 }
 
 Status check_table(const int* table, int64_t stride, int width, int n_seqs) {
     if (width < 0 || stride < 0) return bad("page_table: negative width or stride");
     if (width == 0) return Status::ok();
-    return check_device_pointer(table, (size_t)((n_seqs - 1) * stride + width) * 4, "page_table");
+    return check_pointer(table, (size_t)((n_seqs - 1) * stride + width) * 4, "page_table");
 }
 
 Status do_write(const RtKvWrite& w, void* stream) {
+    t_checked = w.cache.flags & RT_POINTERS_CHECKED;
     CHECK(check_act(w.dtype));
     CHECK(check_cache(w.cache));
     if (w.n_tokens < 0) return bad("kv_write: negative n_tokens");
     if (w.n_tokens == 0) return Status::ok();
     CHECK(check_rows(w.k, w.k_stride, w.n_tokens, w.cache.n_heads, w.cache.head_dim, w.dtype, "kv_write k"));
     CHECK(check_rows(w.v, w.v_stride, w.n_tokens, w.cache.n_heads, w.cache.head_dim, w.dtype, "kv_write v"));
-    CHECK(check_device_pointer(w.slots, (size_t)w.n_tokens * 8, "kv_write slots"));
+    CHECK(check_pointer(w.slots, (size_t)w.n_tokens * 8, "kv_write slots"));
     DeviceGuard g;
     return launch_kv_write(w, static_cast<cudaStream_t>(stream));
 }
 
 Status do_read(const RtKvRead& r, void* stream) {
+    t_checked = r.cache.flags & RT_POINTERS_CHECKED;
     CHECK(check_act(r.dtype));
     CHECK(check_cache(r.cache));
     if (r.n_rows < 0 || r.n_seqs < 0) return bad("kv_read: negative n_rows or n_seqs");
@@ -107,8 +115,8 @@ Status do_read(const RtKvRead& r, void* stream) {
     CHECK(check_rows(r.k_out, r.k_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read k_out"));
     CHECK(check_rows(r.v_out, r.v_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read v_out"));
     CHECK(check_table(r.page_table, r.table_stride, r.table_width, r.n_seqs));
-    if (r.start) CHECK(check_device_pointer(r.start, (size_t)r.n_seqs * 4, "kv_read start"));
-    CHECK(check_device_pointer(r.cu, (size_t)(r.n_seqs + 1) * 4, "kv_read cu"));
+    if (r.start) CHECK(check_pointer(r.start, (size_t)r.n_seqs * 4, "kv_read start"));
+    CHECK(check_pointer(r.cu, (size_t)(r.n_seqs + 1) * 4, "kv_read cu"));
     DeviceGuard g;
     return launch_kv_read(r, static_cast<cudaStream_t>(stream));
 }
@@ -125,6 +133,7 @@ Status check_attention_sizes(const RtPagedAttention& p) {
 }
 
 Status do_attention(const RtPagedAttention& p, void* ws, size_t ws_bytes, void* stream) {
+    t_checked = p.cache.flags & RT_POINTERS_CHECKED;
     CHECK(check_attention_sizes(p));
     CHECK(check_cache(p.cache));
     if (p.total_new == 0 || p.n_seqs == 0) return Status::ok();
@@ -133,21 +142,22 @@ Status do_attention(const RtPagedAttention& p, void* ws, size_t ws_bytes, void* 
     CHECK(check_rows(p.out, p.out_stride, p.total_new, p.n_q_heads, D, p.dtype, "paged_attention out"));
     if ((p.n_q_heads > 1 && p.out_stride[1] < D) || (p.total_new > 1 && p.out_stride[0] < D))
         return bad("paged_attention: rows of out overlap");
-    if (p.lse) CHECK(check_device_pointer(p.lse, (size_t)p.total_new * p.n_q_heads * 4, "paged_attention lse"));
+    if (p.lse) CHECK(check_pointer(p.lse, (size_t)p.total_new * p.n_q_heads * 4, "paged_attention lse"));
     CHECK(check_table(p.page_table, p.table_stride, p.table_width, p.n_seqs));
-    CHECK(check_device_pointer(p.kv_lens, (size_t)p.n_seqs * 4, "paged_attention kv_lens"));
-    CHECK(check_device_pointer(p.cu_new, (size_t)(p.n_seqs + 1) * 4, "paged_attention cu_new"));
+    CHECK(check_pointer(p.kv_lens, (size_t)p.n_seqs * 4, "paged_attention kv_lens"));
+    CHECK(check_pointer(p.cu_new, (size_t)(p.n_seqs + 1) * 4, "paged_attention cu_new"));
     const size_t need = paged_attention_workspace(p);
     if (ws_bytes < need) return bad("paged_attention: workspace of " + std::to_string(ws_bytes) + " bytes, needs " + std::to_string(need));
     if (need) {
         if (!aligned16(ws)) return bad("paged_attention: workspace must be 16-byte aligned");
-        CHECK(check_device_pointer(ws, need, "paged_attention workspace"));
+        CHECK(check_pointer(ws, need, "paged_attention workspace"));
     }
     DeviceGuard g;
     return launch_paged_attention(p, ws, static_cast<cudaStream_t>(stream));
 }
 
 Status do_verify(const RtVerifyDraft& v, void* stream) {
+    t_checked = v.flags & RT_POINTERS_CHECKED;
     CHECK(check_act(v.dtype));
     if (v.n_seqs < 0 || v.n_drafts < 0) return bad("verify_draft: negative count");
     if (v.n_drafts > 1024) return Status::err(RT_ERR_UNSUPPORTED, "verify_draft: more than 1024 drafts");
@@ -157,13 +167,13 @@ Status do_verify(const RtVerifyDraft& v, void* stream) {
     CHECK(check_rows(v.target, v.target_stride, v.n_seqs, v.n_drafts + 1, v.vocab, v.dtype, "verify_draft target"));
     if (v.n_drafts) {
         if (v.draft) CHECK(check_rows(v.draft, v.draft_stride, v.n_seqs, v.n_drafts, v.vocab, v.dtype, "verify_draft draft"));
-        CHECK(check_device_pointer(v.draft_tokens, (size_t)v.n_seqs * v.n_drafts * 4, "verify_draft draft_tokens"));
-        CHECK(check_device_pointer(v.accept_u, (size_t)v.n_seqs * v.n_drafts * 4, "verify_draft accept_u"));
+        CHECK(check_pointer(v.draft_tokens, (size_t)v.n_seqs * v.n_drafts * 4, "verify_draft draft_tokens"));
+        CHECK(check_pointer(v.accept_u, (size_t)v.n_seqs * v.n_drafts * 4, "verify_draft accept_u"));
     }
-    if (v.draft_lens) CHECK(check_device_pointer(v.draft_lens, (size_t)v.n_seqs * 4, "verify_draft draft_lens"));
-    CHECK(check_device_pointer(v.sample_u, (size_t)v.n_seqs * 4, "verify_draft sample_u"));
-    CHECK(check_device_pointer(v.tokens, (size_t)v.n_seqs * (v.n_drafts + 1) * 4, "verify_draft tokens"));
-    CHECK(check_device_pointer(v.accepted, (size_t)v.n_seqs * 4, "verify_draft accepted"));
+    if (v.draft_lens) CHECK(check_pointer(v.draft_lens, (size_t)v.n_seqs * 4, "verify_draft draft_lens"));
+    CHECK(check_pointer(v.sample_u, (size_t)v.n_seqs * 4, "verify_draft sample_u"));
+    CHECK(check_pointer(v.tokens, (size_t)v.n_seqs * (v.n_drafts + 1) * 4, "verify_draft tokens"));
+    CHECK(check_pointer(v.accepted, (size_t)v.n_seqs * 4, "verify_draft accepted"));
     DeviceGuard g;
     return launch_verify_draft(v, static_cast<cudaStream_t>(stream));
 }

@@ -544,13 +544,26 @@ def test_refusals(paged):
     with pytest.raises(TypeError):
         paged.verify_draft(p, p[:, :2].bfloat16(), x, u, u[:, 0].contiguous())
     # a host pointer through the C ABI
-    lib = paged._library(torch.device("cuda", 0))
+    import ctypes
+    from lbr_b200.executor import load_library
+    lib = load_library()
+    lib.rt_kv_write.argtypes, lib.rt_kv_write.restype = [ctypes.POINTER(paged.RtKvWrite), ctypes.c_void_p], ctypes.c_int
     a = paged.RtKvWrite()
-    paged._cache(a.cache, kp, vp, **kw)
+    c = a.cache
+    c.k, c.v, c.k_scale, c.v_scale = kp.data_ptr(), vp.data_ptr(), kw["k_scale"].data_ptr(), kw["v_scale"].data_ptr()
+    c.stride[:], c.scale_stride[:] = kp.stride()[:3], kw["k_scale"].stride()
+    c.dtype, (c.n_pages, c.page_size, c.n_heads, c.head_dim) = 3, kp.shape
+    slots = torch.full((1,), 5, dtype=torch.int64, device="cuda")
+    k = torch.zeros(1, 4, 64, device="cuda")
+    a.k = a.v = k.data_ptr()
+    a.k_stride[:] = a.v_stride[:] = (256, 64)
+    a.slots, a.n_tokens = slots.data_ptr(), 1
+    assert lib.rt_kv_write(a, None) == 0
     host = torch.zeros(1, 4, 64)
-    a.k = a.v = host.data_ptr()
-    a.k_stride[0] = a.v_stride[0] = 256
-    a.k_stride[1] = a.v_stride[1] = 64
-    a.slots, a.n_tokens = s.lens_t.data_ptr(), 1
-    assert lib.rt_kv_write(a, None) in (5, 6)
+    a.k = host.data_ptr()
+    assert lib.rt_kv_write(a, None) == 5            # RT_ERR_HOST_POINTER
+    a.k = None
+    assert lib.rt_kv_write(a, None) == 4            # RT_ERR_NULL_POINTER
+    a.k, a.dtype = k.data_ptr(), 2
+    assert lib.rt_kv_write(a, None) == 7            # RT_ERR_UNSUPPORTED
     paged.check_stream()
