@@ -55,50 +55,56 @@ struct Tile {
     static constexpr int ES = CT == RT_F32 ? 4 : CT == RT_BF16 ? 2 : 1;
     static constexpr bool Q8 = ES == 1;
     static constexpr bool DIRECT = CT == RT_BF16 && !F32ACT;     // bf16 all the way
-    static constexpr bool OWN_SCALE = !DIRECT && !Q8;            // scaled on the way to shared memory
     static constexpr int CHAINS = CT == RT_F32 ? 1 : 2;
     static constexpr int R = 128 * CHAINS;
     static constexpr int QP = F32ACT ? 2 : 1;                    // parts of Q and of P
     static constexpr int VP = CT == RT_F32 ? 2 : 1;              // parts of K and of V
     static constexpr int PLANE = 128 * D * 2;                    // one part of a 128-row tile
     static constexpr int SLOT = VP * PLANE;                      // ring slot
-    static constexpr int SLOTS = CT == RT_F32 ? 2 : F32ACT ? 3 : DIRECT ? 5 : 4;
+    static constexpr int SLOTS = DIRECT ? 5 : F32ACT ? 2 : 3;
+    static constexpr int RB = 4, RAW_PIECE = RB * 128 * 16;      // raw ring: RB loads of 16 bytes a thread
+    static constexpr int NRAW = DIRECT ? 0 : F32ACT ? 3 : 6;
     // Scales are written with their tile and read by its softmax, which may be
-    // behind the loads: by 2 tiles of K and 1 of V with 3 slots, 3 and 1 with 4
-    // (V_j is still held while K_{j+2}, V_{j+1}, K_{j+3} may be loaded).
-    static constexpr int KSD = DIRECT ? 0 : SLOTS == 3 ? 3 : 4, VSD = DIRECT ? 0 : SLOTS == 3 ? 2 : 3;
+    // behind the loads: V_j is still held while K_{j+2} (2 or 3 slots) and
+    // V_{j+1} (3 slots) may be written.
+    static constexpr int KSD = DIRECT ? 0 : 3, VSD = DIRECT ? 0 : 2;
     static constexpr int OFF_RING = CHAINS * QP * PLANE;
-    static constexpr int OFF_KS = OFF_RING + SLOTS * SLOT;
+    static constexpr int OFF_RAW = OFF_RING + SLOTS * SLOT;
+    static constexpr int OFF_RAW_SCALE = OFF_RAW + NRAW * RAW_PIECE;   // by load & 7
+    static constexpr int OFF_KS = OFF_RAW_SCALE + (Q8 ? 4096 : 0);
     static constexpr int OFF_VS = OFF_KS + KSD * 512;
     static constexpr int OFF_BAR = OFF_VS + VSD * 512;
-    static constexpr int SMEM = OFF_BAR + 512;
-    static_assert(SMEM <= 232448, "shared memory");
+    static constexpr int SMEM = OFF_BAR + 1024;
     static constexpr uint32_t COL_S = 0, COL_O = 256;            // + 128 per chain
     static constexpr int OUT = R * D + 2 * R;                    // floats of an unfinished result
+    static_assert(SMEM <= 232448, "shared memory");
 };
 
 struct Bars {
     uint64_t full[5], empty[5];
-    uint64_t s_full[2], p_full[2], q_full[2], join, drain;
+    uint64_t s_full[2], p_full[2], q_full[2], v_notes[4], join, drain;
     uint32_t tmem;
     int abort_flag;
     uint32_t ok[8][4];        // tile T & 7: positions that exist (bit per position)
     float vmax[4][4];         // tile T & 3: largest value scale of each 32 positions
     uint32_t strange[8][4];   // bf16 all the way: positions with values that are not finite
+    uint32_t meta[4][8], there[4][8];   // a loading warp's notes on its loads under way
 };
-static_assert(sizeof(Bars) <= 512, "barrier area");
+static_assert(sizeof(Bars) <= 1024, "barrier area");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     const int n = live ? 16 : 0;   // 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
+    const int n = live ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ void ld_shared16(uint32_t a, uint32_t (&w)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -152,6 +158,11 @@ __device__ __forceinline__ void issue_values(uint32_t d, uint32_t a, uint32_t v,
      ...);
 }
 
+// A wait of a whole warp: all its lanes go on, or none.
+__device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+    return __all_sync(0xffffffffu, ptx::wait_bounded(b, parity, abort_flag, err, code, WAIT_NS));
+}
+
 // What every role walks through: the block's segments.
 struct Segment {
     int tiles, k0;        // key tiles, first position of the first
@@ -196,6 +207,8 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             ptx::mbar_init(&bar.s_full[i], 1);
             ptx::mbar_init(&bar.p_full[i], 128);
             ptx::mbar_init(&bar.q_full[i], 128);
+            ptx::mbar_init(&bar.v_notes[i], 128);
+            ptx::mbar_init(&bar.v_notes[2 + i], 128);
         }
         ptx::mbar_init(&bar.join, 256);
         ptx::mbar_init(&bar.drain, 1);
@@ -212,215 +225,231 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
 
     if (warp < 4) {
         // ------------------------------------------------ K and V from the pages
+        // A lane looks up one position of the warp's 32, all lanes then copy rows:
+        // cp.async, straight into the ring (bf16 all the way) or, in pieces of RB
+        // loads a lane, into a raw ring from which the same thread converts its own
+        // bytes.  Copies run AHEAD pieces in front of what is handed over.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_LOAD));
-        int n_load = 0, tile_base = 0;    // loads so far (slot n_load % SLOTS), tiles before this segment
         bool ok = true;
-        const uint32_t ring = ptx::smem_u32(smem + T::OFF_RING);
-        constexpr int LAG = T::DIRECT ? T::SLOTS - 2 : 0;   // copies in flight behind the newest
+        const uint32_t ring = ptx::smem_u32(smem + T::OFF_RING), raw = ptx::smem_u32(smem + T::OFF_RAW) + tid * 16;
         constexpr int LANES = D * T::ES / 16, ROWS = 32 / LANES;          // lanes of a row, rows of a warp's load
-        constexpr int LOADS = 32 / ROWS, BATCH = LOADS < 8 ? LOADS : 8;   // loads of a warp's 32 rows; in flight together
-        const int sub_row = lane / LANES, piece = lane % LANES;
-        auto publish = [&](int load) {
-            ptx::fence_proxy_async_smem();
-            ptx::mbar_arrive(&bar.full[load % T::SLOTS]);
-        };
-        // checked: the V copies of tiles that rows see differently (DIRECT): load -> tile, -1 none
-        auto clean_v = [&](int load, int tile_no) {
-            const uint32_t at = ring + (uint32_t)(load % T::SLOTS) * T::SLOT;
-#pragma unroll 1
-            for (int i = 0; i < LOADS; i++) {
-                const int r = warp * 32 + i * ROWS + sub_row;
-                const uint32_t a = at + tile_at(r, piece * 16);
-                uint32_t w[4];
-                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
-                bool found = false;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, found = true;
-                    if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, found = true;
-                }
-                if (found) {
-                    st_shared16(a, w[0], w[1], w[2], w[3]);
-                    atomicOr(&bar.strange[tile_no & 7][r >> 5], 1u << (r & 31));
-                }
-            }
-        };
-        int check_tile[8];   // by load & 7
-#pragma unroll
-        for (int i = 0; i < 8; i++) check_tile[i] = -1;
+        constexpr int LOADS = 32 / ROWS;                                  // loads of a warp's 32 rows
+        constexpr int PIECES = T::DIRECT ? 1 : LOADS / T::RB, PER = LOADS / PIECES;
+        constexpr int AHEAD = T::DIRECT ? T::SLOTS - 2 : T::NRAW - 1;
+        const int sub_row = lane / LANES, piece16 = lane % LANES;
+        volatile uint32_t* meta = bar.meta[warp];                         // by load & 7: is_v | mixed << 1 | tile << 2
+        volatile uint32_t* there = bar.there[warp];                       // by load & 7: positions that exist
 
-        while (ok && u < u_end) {
-            const Segment g = segment_of<T>(p, cur, u, u_end);
-            const uint8_t* kb = static_cast<const uint8_t*>(c.k) + cur.h * c.stride[2] * T::ES;
-            const uint8_t* vb = static_cast<const uint8_t*>(c.v) + cur.h * c.stride[2] * T::ES;
-            const int* table = p.a.page_table + cur.s.b * p.a.table_stride;
-            // positions seen by every row of the item
-            const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = cur.s.L - cur.s.n;
-            const int all_hi = p.a.causal ? min(cur.s.L, at0 + tok0 + 1) : cur.s.L;
-            const int all_lo = p.a.window > 0 ? max(0, at0 + tok1 - p.a.window + 1) : 0;
-
-            auto load = [&](bool is_v, int j) {
-                const int pos = g.k0 + j * TKT + warp * 32 + lane, tile_no = tile_base + j;
-                int64_t off = -1;
-                float scale = 0.0f;
-                if (pos >= cur.t.lo && pos < cur.t.hi) {
+        // ---- the copies ----
+        Segment g = segment_of<T>(p, cur, u, u_end);
+        int idx = 0, tile_base = 0, n_copy = 0, part = 0;   // load of the segment, tiles before it, loads begun, piece
+        uint32_t off0 = ~0u, off1 = ~0u, off_now = ~0u;     // this lane's row of even / odd tiles, units of 16 bytes
+        int sp0 = 0, sp1 = 0, sp_now = 0, page_next = 0;    // its scale; the page of the next key tile
+        bool is_v = false;
+        auto page_of = [&](int j) -> int {
+            const int pos = g.k0 + j * TKT + warp * 32 + lane;
+            if (pos < cur.t.lo || pos >= cur.t.hi) return -1;
+            int ip, slot;
+            paged_split(p, pos, ip, slot);
+            const int page = p.a.page_table[cur.s.b * p.a.table_stride + ip];
+            return page < 0 ? 0x7fffffff : page;
+        };
+        auto begin_load = [&]() {
+            const int a = (T::CHAINS == 2 && !g.two) ? 2 : 1, n = g.tiles, head = min(a, n), r = idx - head, both = max(0, n - a);
+            int j;   // K0 (K1) | V0 K(a) | V1 K(a+1) | ... | the last V
+            if (r < 0) is_v = false, j = idx;
+            else if (r < 2 * both) is_v = !(r & 1), j = (r >> 1) + (r & 1 ? a : 0);
+            else is_v = true, j = both + r - 2 * both;
+            if (idx == 0) page_next = page_of(0);
+            if (!is_v) {
+                const int pos = g.k0 + j * TKT + warp * 32 + lane;
+                uint32_t off = ~0u;
+                int sp = 0;
+                if (page_next >= c.n_pages) {
+                    atomicCAS(p.err, 0, KERR_PAGE);
+                } else if (page_next >= 0) {
                     int ip, slot;
                     paged_split(p, pos, ip, slot);
-                    const int page = table[ip];
-                    if (page >= 0 && page < c.n_pages) {
-                        off = (page * c.stride[0] + slot * c.stride[1]) * T::ES;
-                        if constexpr (T::Q8)
-                            scale = __ldg((is_v ? c.v_scale : c.k_scale) + page * c.scale_stride[0] + slot * c.scale_stride[1] + cur.h * c.scale_stride[2]);
-                    } else {
-                        atomicCAS(p.err, 0, KERR_PAGE);
+                    off = (uint32_t)((page_next * c.stride[0] + slot * c.stride[1] + cur.h * c.stride[2]) * T::ES >> 4);
+                    if constexpr (T::Q8) sp = (int)(page_next * c.scale_stride[0] + slot * c.scale_stride[1] + cur.h * c.scale_stride[2]);
+                }
+                if (j + 1 < n) page_next = page_of(j + 1);
+                if (j & 1) off1 = off, sp1 = sp;
+                else off0 = off, sp0 = sp;
+            }
+            off_now = j & 1 ? off1 : off0;
+            sp_now = j & 1 ? sp1 : sp0;
+            const uint32_t live = __ballot_sync(0xffffffffu, off_now != ~0u);
+            bool mixed = false;
+            if constexpr (T::DIRECT) {   // does every row of the item see all of this tile?
+                const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = cur.s.L - cur.s.n, k = g.k0 + j * TKT;
+                mixed = is_v && tok1 > tok0 && ((p.a.causal && k + TKT > at0 + tok0 + 1) || (p.a.window > 0 && k < at0 + tok1 - p.a.window + 1));
+            }
+            if (lane == 0) {
+                meta[n_copy & 7] = (is_v ? 1u : 0u) | (mixed ? 2u : 0u) | (uint32_t)(tile_base + j) << 2;
+                there[n_copy & 7] = live;
+            }
+        };
+        auto copy_piece = [&]() {
+            if (part == 0) begin_load();
+            uint32_t dst;
+            if constexpr (T::DIRECT) {
+                const int s = n_copy % T::SLOTS;
+                if (n_copy >= T::SLOTS)
+                    ok = wait_warp(&bar.empty[s], (n_copy / T::SLOTS - 1) & 1, abort_flag, p.err, ERR_P_LOAD);
+                if (!ok) return;
+                dst = ring + (uint32_t)s * T::SLOT;
+            } else {
+                dst = raw + (uint32_t)((n_copy * PIECES + part) % T::NRAW) * T::RAW_PIECE;
+            }
+            const uint8_t* base = static_cast<const uint8_t*>(is_v ? c.v : c.k);
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int r = (part * PER + i) * ROWS + sub_row;
+                const uint32_t o = __shfl_sync(0xffffffffu, off_now, r);
+                const uint8_t* src = base + ((uint64_t)(o == ~0u ? 0 : o) << 4) + piece16 * 16;
+                cp_async16(T::DIRECT ? dst + tile_at(warp * 32 + r, piece16 * 16) : dst + i * 2048, src, o != ~0u);
+            }
+            if constexpr (T::Q8)
+                if (part == 0)
+                    cp_async4(ptx::smem_u32(smem + T::OFF_RAW_SCALE) + ((n_copy & 7) * 128 + tid) * 4, (is_v ? c.v_scale : c.k_scale) + sp_now,
+                              off_now != ~0u);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (++part == PIECES) {
+                part = 0;
+                n_copy++;
+                if (++idx == 2 * g.tiles) {
+                    idx = 0;
+                    tile_base += g.tiles;
+                    u += g.tiles;
+                    cur.next_item<T::R, TKT>(p);
+                    if (u < u_end) g = segment_of<T>(p, cur, u, u_end);
+                }
+            }
+        };
+        // ---- handing over ----
+        int n_done = 0, done_part = 0;
+        uint32_t top_all = 0;   // own scales: the largest of this lane's rows (bits)
+        auto hand_piece = [&]() {
+            const uint32_t what = meta[n_done & 7], live = there[n_done & 7];
+            const bool v = what & 1;
+            const int tile_no = (int)(what >> 2), s = n_done % T::SLOTS;
+            const uint32_t dst = ring + (uint32_t)s * T::SLOT;
+            if (!v && done_part == 0 && lane == 0) bar.ok[tile_no & 7][warp] = live;
+            if constexpr (T::DIRECT) {
+                if (v && warp == 0 && lane < 4) bar.strange[(tile_no + 4) & 7][lane] = 0;   // four tiles ahead of its use
+                if (what & 2) {
+                    // Rows of the item see this tile differently: values that are not finite
+                    // leave it (0 times them is not 0) and their positions are noted.
+#pragma unroll 1
+                    for (int i = 0; i < LOADS; i++) {
+                        const int r = warp * 32 + i * ROWS + sub_row;
+                        const uint32_t at = dst + tile_at(r, piece16 * 16);
+                        uint32_t w[4];
+                        ld_shared16(at, w);
+                        bool found = false;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, found = true;
+                            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, found = true;
+                        }
+                        if (found) {
+                            st_shared16(at, w[0], w[1], w[2], w[3]);
+                            atomicOr(&bar.strange[tile_no & 7][r >> 5], 1u << (r & 31));
+                        }
                     }
                 }
-                const uint8_t* base = is_v ? vb : kb;
-                const int slot_no = n_load % T::SLOTS;
-                const uint32_t dst = ring + (uint32_t)slot_no * T::SLOT;
-                float* scales = is_v ? reinterpret_cast<float*>(smem + T::OFF_VS) + tile_no % (T::VSD ? T::VSD : 1) * 128
-                                     : reinterpret_cast<float*>(smem + T::OFF_KS) + tile_no % (T::KSD ? T::KSD : 1) * 128;
-                auto wait_slot = [&]() {
-                    if (n_load >= T::SLOTS)
-                        ok = ptx::wait_bounded(&bar.empty[slot_no], (n_load / T::SLOTS - 1) & 1, abort_flag, p.err, ERR_P_LOAD, WAIT_NS);
-                };
-                if constexpr (T::DIRECT) {
-                    wait_slot();
+            } else {
+                float* scales = v ? reinterpret_cast<float*>(smem + T::OFF_VS) + tile_no % T::VSD * 128
+                                  : reinterpret_cast<float*>(smem + T::OFF_KS) + tile_no % T::KSD * 128;
+                if (done_part == 0) {
+                    if (n_done >= T::SLOTS)
+                        ok = wait_warp(&bar.empty[s], (n_done / T::SLOTS - 1) & 1, abort_flag, p.err, ERR_P_LOAD);
                     if (!ok) return;
-                    const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
-                    if (!is_v && lane == 0) bar.ok[tile_no & 7][warp] = there;
-                    if (is_v && warp == 0 && lane < 4) bar.strange[(tile_no + 4) & 7][lane] = 0;   // four tiles ahead of its use
-#pragma unroll
-                    for (int i = 0; i < LOADS; i++) {
-                        const int r = i * ROWS + sub_row;
-                        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                        cp_async16(dst + tile_at(warp * 32 + r, piece * 16), base + (o >= 0 ? o : 0) + piece * 16, o >= 0);
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    const int k = g.k0 + j * TKT;
-                    const bool mixed = is_v && (k + TKT > all_hi || k < all_lo) && tok1 > tok0;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i == (n_load & 7)) check_tile[i] = mixed ? tile_no : -1;
-                    if (n_load >= LAG) {
-                        cp_wait<LAG>();
-                        int ct = -1;
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            if (i == ((n_load - LAG) & 7)) ct = check_tile[i];
-                        if (ct >= 0) clean_v(n_load - LAG, ct);
-                        publish(n_load - LAG);
-                    }
-                } else {
-                    uint4 x[BATCH];
-                    auto fetch = [&](int i0) {
-#pragma unroll
-                        for (int i = 0; i < BATCH; i++) {
-                            const int64_t o = __shfl_sync(0xffffffffu, off, (i0 + i) * ROWS + sub_row);
-                            x[i] = make_uint4(0, 0, 0, 0);
-                            if (o >= 0) x[i] = ld_stream(base + o + piece * 16);
-                        }
-                    };
-                    fetch(0);
-                    wait_slot();
-                    if (!ok) return;
-                    const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
-                    if (!is_v && lane == 0) bar.ok[tile_no & 7][warp] = there;
+                    top_all = 0;
                     if constexpr (T::Q8) {
-                        scales[warp * 32 + lane] = scale;
-                        if (is_v) {
-                            float top = scale;
-#pragma unroll
-                            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            if (lane == 0) bar.vmax[tile_no & 3][warp] = top;
-                        }
+                        const float scale = *reinterpret_cast<const volatile float*>(smem + T::OFF_RAW_SCALE + ((n_done & 7) * 128 + tid) * 4);
+                        scales[tid] = scale;
+                        if (scale > 0.0f && scale < INFINITY) top_all = __float_as_uint(scale);
                     }
-                    float top_all = 0.0f;   // own scales: the largest of this lane's rows
+                }
+                const uint32_t src = raw + (uint32_t)((n_done * PIECES + done_part) % T::NRAW) * T::RAW_PIECE;
 #pragma unroll
-                    for (int i0 = 0; i0 < LOADS; i0 += BATCH) {
-                        if (i0) fetch(i0);
+                for (int i = 0; i < PER; i++) {
+                    const int r = warp * 32 + (done_part * PER + i) * ROWS + sub_row;
+                    uint32_t w[4];
+                    ld_shared16(src + i * 2048, w);
+                    if constexpr (T::Q8) {
+                        uint32_t h[8];
 #pragma unroll
-                        for (int i = 0; i < BATCH; i++) {
-                            const int r = warp * 32 + (i0 + i) * ROWS + sub_row;
-                            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                            if constexpr (T::Q8) {
-                                uint32_t h[8];
+                        for (int k = 0; k < 4; k++) codes_f16<CT>(w[k], h[2 * k], h[2 * k + 1]);
+                        st_shared16(dst + tile_at(r, piece16 * 32), h[0], h[1], h[2], h[3]);
+                        st_shared16(dst + tile_at(r, piece16 * 32 + 16), h[4], h[5], h[6], h[7]);
+                    } else {
+                        constexpr int N = 16 / T::ES;
+                        float x[N];
 #pragma unroll
-                                for (int k = 0; k < 4; k++) codes_f16<CT>(w[k], h[2 * k], h[2 * k + 1]);
-                                st_shared16(dst + tile_at(r, piece * 32), h[0], h[1], h[2], h[3]);
-                                st_shared16(dst + tile_at(r, piece * 32 + 16), h[4], h[5], h[6], h[7]);
+                        for (int k = 0; k < 4; k++) {
+                            if constexpr (CT == RT_BF16) {
+                                x[2 * k] = __uint_as_float(w[k] << 16);
+                                x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
                             } else {
-                                constexpr int N = 16 / T::ES;
-                                float v[N];
-#pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    if constexpr (CT == RT_BF16) {
-                                        v[2 * k] = __uint_as_float(w[k] << 16);
-                                        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-                                    } else {
-                                        v[k] = __uint_as_float(w[k]);
-                                    }
-                                }
-                                uint32_t top = 0;   // over the bits of |x|: what is not finite comes out on top
-#pragma unroll
-                                for (int k = 0; k < N; k++) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
-#pragma unroll
-                                for (int o = LANES / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                                const int e = f16_scale_exp(__uint_as_float(top));
-                                const bool finite = top < 0x7f800000u;
-                                const float up = finite ? pow2i(e) : 0.0f;
-                                const float down = finite ? pow2i(-e) : __uint_as_float(0x7fc00000u);
-#pragma unroll
-                                for (int k = 0; k < N; k++) v[k] = finite ? v[k] * up : 0.0f;
-                                if (piece == 0) scales[r] = down;
-                                if (finite && top) top_all = fmaxf(top_all, down);
-                                if constexpr (T::VP == 1) {
-                                    st_shared16(dst + tile_at(r, piece * 16), f16x2_rn(v[0], v[1]), f16x2_rn(v[2], v[3]),
-                                                f16x2_rn(v[4 % N], v[5 % N]), f16x2_rn(v[6 % N], v[7 % N]));
-                                } else {
-                                    float h[4];
-#pragma unroll
-                                    for (int k = 0; k < 4; k++) h[k] = round11(v[k]);
-                                    const uint32_t at = dst + tile_at(r, piece * 8);
-                                    st_shared8(at, f16x2_rn(h[0], h[1]), f16x2_rn(h[2], h[3]));
-                                    st_shared8(at + T::PLANE, f16x2_rn(v[0] - h[0], v[1] - h[1]), f16x2_rn(v[2] - h[2], v[3] - h[3]));
-                                }
+                                x[k] = __uint_as_float(w[k]);
                             }
                         }
-                    }
-                    if constexpr (T::OWN_SCALE)
-                        if (is_v) {
+                        uint32_t top = 0;   // over the bits of |x|: what is not finite comes out on top
 #pragma unroll
-                            for (int o = 16; o; o >>= 1) top_all = fmaxf(top_all, __shfl_xor_sync(0xffffffffu, top_all, o));
-                            if (lane == 0) bar.vmax[tile_no & 3][warp] = top_all;
+                        for (int k = 0; k < N; k++) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+#pragma unroll
+                        for (int o = LANES / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const int e = f16_scale_exp(__uint_as_float(top));
+                        const bool finite = top < 0x7f800000u;
+                        const float up = finite ? pow2i(e) : 0.0f;
+                        const float down = finite ? pow2i(-e) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+                        for (int k = 0; k < N; k++) x[k] = finite ? x[k] * up : 0.0f;
+                        if (piece16 == 0) scales[r] = down;
+                        if (finite && top) top_all = max(top_all, __float_as_uint(down));
+                        if constexpr (T::VP == 1) {
+                            st_shared16(dst + tile_at(r, piece16 * 16), f16x2_rn(x[0], x[1]), f16x2_rn(x[2], x[3]),
+                                        f16x2_rn(x[4 % N], x[5 % N]), f16x2_rn(x[6 % N], x[7 % N]));
+                        } else {
+                            float h[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) h[k] = round11(x[k]);
+                            const uint32_t at = dst + tile_at(r, piece16 * 8);
+                            st_shared8(at, f16x2_rn(h[0], h[1]), f16x2_rn(h[2], h[3]));
+                            st_shared8(at + T::PLANE, f16x2_rn(x[0] - h[0], x[1] - h[1]), f16x2_rn(x[2] - h[2], x[3] - h[3]));
                         }
-                    publish(n_load);
+                    }
                 }
-                n_load++;
-            };
-            // in the order the products take them
-            const int ahead = (T::CHAINS == 2 && !g.two) ? 2 : 1;
-            for (int j = 0; j < min(ahead, g.tiles) && ok; j++) load(false, j);
-            for (int j = 0; j < g.tiles && ok; j++) {
-                load(true, j);
-                if (ok && j + ahead < g.tiles) load(false, j + ahead);
+                if (v && done_part == PIECES - 1) {
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, top_all);
+                    if (lane == 0) bar.vmax[tile_no & 3][warp] = __uint_as_float(top);
+                }
             }
-            tile_base += g.tiles;
-            u += g.tiles;
-            cur.next_item<T::R, TKT>(p);
+            if (++done_part == PIECES) {
+                done_part = 0;
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(&bar.full[s]);
+                if (v) ptx::mbar_arrive(&bar.v_notes[tile_no & 3]);
+                n_done++;
+            }
+        };
+        int ahead = 0;
+        while (ok && u < u_end) {
+            copy_piece();
+            if (!ok) break;
+            if (++ahead > AHEAD) {
+                cp_wait<AHEAD>();
+                __syncwarp();
+                hand_piece();
+                ahead--;
+            }
         }
-        if constexpr (T::DIRECT) {   // the copies still in flight
-            cp_wait<0>();
-            if (ok)
-                for (int l = max(0, n_load - LAG); l < n_load; l++) {
-                    int ct = -1;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i == (l & 7)) ct = check_tile[i];
-                    if (ct >= 0) clean_v(l, ct);
-                    publish(l);
-                }
-        }
+        cp_wait<0>();
+        __syncwarp();
+        for (; ok && ahead > 0; ahead--) hand_piece();
     } else if (warp < 8) {
         // ------------------------------------------------ MMA issue
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_MMA));
@@ -535,15 +564,15 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_at = tmem + lanes + T::COL_S + chain * 128, o_at = tmem + lanes + T::COL_O + chain * 128;
         const float base = p.a.scale * 1.4426950408889634f;
-        int n_s = 0, n_join = 0, tile_base = 0, load_base = 0;
+        int n_s = 0, n_join = 0, tile_base = 0;
         bool ok = true, was_two = false;
         auto wait_s = [&]() {
-            ok = ptx::wait_bounded(&bar.s_full[chain], n_s++ & 1, abort_flag, p.err, ERR_P_SOFT, WAIT_NS);
+            ok = wait_warp(&bar.s_full[chain], n_s++ & 1, abort_flag, p.err, ERR_P_SOFT);
             ptx::tc_fence_after();
         };
         auto meet = [&]() {   // both chains' softmax threads
             ptx::mbar_arrive(&bar.join);
-            ok = ptx::wait_bounded(&bar.join, n_join++ & 1, abort_flag, p.err, ERR_P_SOFT, WAIT_NS);
+            ok = wait_warp(&bar.join, n_join++ & 1, abort_flag, p.err, ERR_P_SOFT);
         };
         while (ok && u < u_end) {
             const Segment g = segment_of<T>(p, cur, u, u_end);
@@ -653,15 +682,16 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                     wait_s();
                     if (!ok) break;
                     if (j == j0 && split_keys && chain == 1 && !T::DIRECT) c_row = reinterpret_cast<const float*>(q1)[row];
-                    // What comes with V_j (its scales, the positions taken out of it) is there
-                    // once V_j has landed, which its product waits for, not the scores.
+                    // What comes with V_j (its scales, the positions taken out of it) is there once
+                    // V_j has landed, which its product waits for, not the scores.  (Not the ring
+                    // slot's barrier, which may be two phases away here: up to two later V
+                    // tiles may have landed too, hence four barriers.)
                     auto wait_v = [&]() {
-                        const int load = load_base + min(j + (split_keys ? 2 : 1), g.tiles) + j;
-                        ok = ptx::wait_bounded(&bar.full[load % T::SLOTS], (load / T::SLOTS) & 1, abort_flag, p.err, ERR_P_SOFT, WAIT_NS);
+                        ok = wait_warp(&bar.v_notes[tile_no & 3], (tile_no >> 2) & 1, abort_flag, p.err, ERR_P_SOFT);
                     };
                     if (any_live) {
-                        const float* ks = reinterpret_cast<const float*>(smem + T::OFF_KS) + tile_no % (T::KSD ? T::KSD : 1) * 128;
-                        const float* vs = reinterpret_cast<const float*>(smem + T::OFF_VS) + tile_no % (T::VSD ? T::VSD : 1) * 128;
+                        const float* ks = reinterpret_cast<const float*>(smem + T::OFF_KS) + tile_no % (T::DIRECT ? 1 : T::KSD) * 128;
+                        const float* vs = reinterpret_cast<const float*>(smem + T::OFF_VS) + tile_no % (T::DIRECT ? 1 : T::VSD) * 128;
                         const uint32_t* okw = bar.ok[tile_no & 7];
                         const bool whole = lo_row <= k0 && hi_row >= k0 + TKT && (okw[0] & okw[1] & okw[2] & okw[3]) == 0xffffffffu;
                         const bool masked = __any_sync(0xffffffffu, live && !whole);
@@ -864,7 +894,6 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 }
             }
             tile_base += g.tiles;
-            load_base += 2 * g.tiles;
             u += g.tiles;
             cur.next_item<T::R, TKT>(p);
         }
