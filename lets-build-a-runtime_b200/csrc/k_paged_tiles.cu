@@ -3,17 +3,18 @@
 //
 // Tiles of 128 rows (new token x query head of one cache head) x 128 cached
 // positions: S = Q.K^T into TMEM, weights P = 2^(S c - m) back into TMEM over
-// S, O = P.V with A from TMEM.  Two chains of tiles run in every block, so that
-// one chain's softmax works while the tensor cores run the other's products:
-//   more than 128 rows: chain t takes rows 128 t .. of the item's 256, both go
-//     over all key tiles;
-//   up to 128 rows: both chains have the same rows and take alternate key
-//     tiles, each with its own maximum; they are added up at the end of the item.
+// S, O = P.V with A from TMEM.  S, P and O exist twice, so that softmax works on
+// one while the tensor cores run the other's products:
+//   bf16 activations, more than 128 rows: two row tiles over the same key tiles,
+//     a warpgroup each;
+//   bf16 activations, up to 128 rows: one row tile, a warpgroup takes every other
+//     key tile with a maximum of its own; the two are added at the end of the item;
+//   fp32 activations: one row tile, both warpgroups on every key tile, each half
+//     of its positions (a row's sums need the registers of two threads).
 // 512 threads: warps 0-3 fetch K and V from the pages into a ring of shared
 // memory tiles (128-byte swizzle; K as [position][64 features], which is
 // K-major for Q.K^T, V the same, which is MN-major for P.V -- nothing is
-// transposed), warp 4 issues the MMAs, warps 8-11 and 12-15 are the softmax of
-// chains 0 and 1, a thread per row.
+// transposed), warp 4 issues the MMAs, warps 8-15 are the softmax.
 //
 // Operands.  bf16 activations over a bf16 cache: cp.async straight from the
 // pages, bf16 products.  Everything else becomes fp16 on the way to shared
@@ -24,8 +25,9 @@
 // reference m carries the largest value scale seen, so weights stay in fp16's
 // range.  fp32 activations: Q and P as fp16 hi + lo (22 bits), an fp32 cache's
 // K and V as well: 2 or 3 products for one.  bf16 activations: one part each.
-// The tensor core's own sum truncates, so O is folded into fp32 registers
-// after every key tile.
+// The tensor core's own sum truncates (2^-24 of the sum per step, always down):
+// with bf16 outputs that is nothing even over long caches and O stays in TMEM,
+// with fp32 outputs every key tile's O is folded into fp32 registers.
 //
 // Bound: tensor pipe and exponentials for long chunks (a 128 x 128 tile pair
 // of products is 1024 cycles at D = 128, its 16384 exponentials 1024 as well),
@@ -55,34 +57,35 @@ struct Tile {
     static constexpr int ES = CT == RT_F32 ? 4 : CT == RT_BF16 ? 2 : 1;
     static constexpr bool Q8 = ES == 1;
     static constexpr bool DIRECT = CT == RT_BF16 && !F32ACT;     // bf16 all the way
-    static constexpr int CHAINS = CT == RT_F32 ? 1 : 2;
-    static constexpr int R = 128 * CHAINS;
+    static constexpr int R = F32ACT ? 128 : 256;                 // rows of an item
     static constexpr int QP = F32ACT ? 2 : 1;                    // parts of Q and of P
     static constexpr int VP = CT == RT_F32 ? 2 : 1;              // parts of K and of V
     static constexpr int PLANE = 128 * D * 2;                    // one part of a 128-row tile
     static constexpr int SLOT = VP * PLANE;                      // ring slot
-    static constexpr int SLOTS = DIRECT ? 5 : F32ACT ? 2 : 3;
+    static constexpr int SLOTS = DIRECT ? 5 : VP == 2 ? 2 : 3;
     static constexpr int RB = 4, RAW_PIECE = RB * 128 * 16;      // raw ring: RB loads of 16 bytes a thread
-    static constexpr int NRAW = DIRECT ? 0 : F32ACT ? 3 : 6;
+    static constexpr int NRAW = DIRECT ? 0 : VP == 2 ? 3 : 6;
     // Scales are written with their tile and read by its softmax, which may be
     // behind the loads: V_j is still held while K_{j+2} (2 or 3 slots) and
     // V_{j+1} (3 slots) may be written.
     static constexpr int KSD = DIRECT ? 0 : 3, VSD = DIRECT ? 0 : 2;
-    static constexpr int OFF_RING = CHAINS * QP * PLANE;
+    static constexpr int OFF_RING = R / 128 * QP * PLANE;
     static constexpr int OFF_RAW = OFF_RING + SLOTS * SLOT;
     static constexpr int OFF_RAW_SCALE = OFF_RAW + NRAW * RAW_PIECE;   // by load & 7
     static constexpr int OFF_KS = OFF_RAW_SCALE + (Q8 ? 4096 : 0);
     static constexpr int OFF_VS = OFF_KS + KSD * 512;
-    static constexpr int OFF_BAR = OFF_VS + VSD * 512;
+    static constexpr int OFF_QS = OFF_VS + VSD * 512;                  // per row: scale of a score
+    static constexpr int OFF_RED = OFF_QS + (DIRECT ? 0 : R * 4);      // fp32 activations: [2][2][128] maxima of half rows
+    static constexpr int OFF_BAR = OFF_RED + (F32ACT ? 2048 : 0);
     static constexpr int SMEM = OFF_BAR + 1024;
-    static constexpr uint32_t COL_S = 0, COL_O = 256;            // + 128 per chain
+    static constexpr uint32_t COL_S = 0, COL_O = 256;            // + 128 for the second
     static constexpr int OUT = R * D + 2 * R;                    // floats of an unfinished result
     static_assert(SMEM <= 232448, "shared memory");
 };
 
 struct Bars {
     uint64_t full[5], empty[5];
-    uint64_t s_full[2], p_full[2], q_full[2], v_notes[4], join, drain;
+    uint64_t s_full[2], p_full[2], q_full[2], v_notes[4], join, half[4], drain;
     uint32_t tmem;
     int abort_flag;
     uint32_t ok[8][4];        // tile T & 7: positions that exist (bit per position)
@@ -136,7 +139,7 @@ __device__ __forceinline__ uint32_t bf16_pair_rn(float a, float b) {
 }
 
 // One product over all K steps.  P lies over S: per 16 positions 8 columns of
-// hi pairs, then 8 of lo pairs.
+// hi pairs, then (two parts) 8 of lo pairs.
 template <class T, int D, int... I>
 __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t q, uint32_t k, uint32_t kind, std::integer_sequence<int, I...>) {
     (([&] {
@@ -148,12 +151,12 @@ __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t q, uint32_t k,
      ...);
 }
 template <class T, int... I>
-__device__ __forceinline__ void issue_values(uint32_t d, uint32_t a, uint32_t v, uint32_t kind, std::integer_sequence<int, I...>) {
+__device__ __forceinline__ void issue_values(uint32_t d, uint32_t a, uint32_t v, uint32_t kind, uint32_t add, std::integer_sequence<int, I...>) {
     (([&] {
-         constexpr uint32_t o = I * 2048 >> 4, part = T::PLANE >> 4;
-         ptx::mma_f16_ts<I * 16, o>(d, a, v, kind, I ? 1u : 0u);
-         if constexpr (T::QP == 2) ptx::mma_f16_ts<I * 16 + 8, o>(d, a, v, kind, 1u);
-         if constexpr (T::VP == 2) ptx::mma_f16_ts<I * 16, o + part>(d, a, v, kind, 1u);
+         constexpr uint32_t o = I * 2048 >> 4, part = T::PLANE >> 4, col = I * 8 * T::QP;
+         ptx::mma_f16_ts<col, o>(d, a, v, kind, I ? 1u : add);
+         if constexpr (T::QP == 2) ptx::mma_f16_ts<col + 8, o>(d, a, v, kind, 1u);
+         if constexpr (T::VP == 2) ptx::mma_f16_ts<col, o + part>(d, a, v, kind, 1u);
      }()),
      ...);
 }
@@ -176,7 +179,7 @@ __device__ __forceinline__ Segment segment_of(const PagedArgs& p, const PagedCur
     g.k0 = (c.t.t0 + c.i) * TKT;
     g.row0 = c.qt * T::R;
     g.rows = min(T::R, c.s.n * p.group - g.row0);
-    g.two = T::CHAINS == 2 && g.rows > 128;
+    g.two = T::R == 256 && g.rows > 128;
     return g;
 }
 
@@ -205,12 +208,13 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
         }
         for (int i = 0; i < 2; i++) {
             ptx::mbar_init(&bar.s_full[i], 1);
-            ptx::mbar_init(&bar.p_full[i], 128);
-            ptx::mbar_init(&bar.q_full[i], 128);
+            ptx::mbar_init(&bar.p_full[i], F32ACT ? 256 : 128);
+            ptx::mbar_init(&bar.q_full[i], F32ACT ? 256 : 128);
             ptx::mbar_init(&bar.v_notes[i], 128);
             ptx::mbar_init(&bar.v_notes[2 + i], 128);
         }
         ptx::mbar_init(&bar.join, 256);
+        for (int i = 0; i < 4; i++) ptx::mbar_init(&bar.half[i], 64);
         ptx::mbar_init(&bar.drain, 1);
         bar.abort_flag = 0;
         for (int i = 0; i < 8; i++)
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             return page < 0 ? 0x7fffffff : page;
         };
         auto begin_load = [&]() {
-            const int a = (T::CHAINS == 2 && !g.two) ? 2 : 1, n = g.tiles, head = min(a, n), r = idx - head, both = max(0, n - a);
+            const int a = g.two ? 1 : 2, n = g.tiles, head = min(a, n), r = idx - head, both = max(0, n - a);
             int j;   // K0 (K1) | V0 K(a) | V1 K(a+1) | ... | the last V
             if (r < 0) is_v = false, j = idx;
             else if (r < 2 * both) is_v = !(r & 1), j = (r >> 1) + (r & 1 ? a : 0);
@@ -469,9 +473,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 issue_scores<T, D>(tmem + T::COL_S + chain * 128, q_desc + (uint32_t)(q_tile * (T::QP * T::PLANE >> 4)),
                                    k_desc + (uint32_t)(load % T::SLOTS * (T::SLOT >> 4)), kind_s, std::make_integer_sequence<int, D / 16>());
             };
-            auto values = [&](int chain, int load) {   // O = P.V over 128 positions
+            auto values = [&](int chain, int load, bool add) {   // O (+)= P.V over 128 positions
                 issue_values<T>(tmem + T::COL_O + chain * 128, tmem + T::COL_S + chain * 128,
-                                v_desc + (uint32_t)(load % T::SLOTS * (T::SLOT >> 4)), kind_o, std::make_integer_sequence<int, TKT / 16>());
+                                v_desc + (uint32_t)(load % T::SLOTS * (T::SLOT >> 4)), kind_o, add ? 1u : 0u,
+                                std::make_integer_sequence<int, TKT / 16>());
             };
             auto wait_p = [&](int chain) {
                 if (ok) ok = ptx::wait_bounded(&bar.p_full[chain], n_p[chain]++ & 1, abort_flag, p.err, ERR_P_MMA, WAIT_NS);
@@ -485,7 +490,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 const Segment g = segment_of<T>(p, cur, u, u_end);
                 wait_q(0);
                 if (g.two) wait_q(1);
-                if (T::CHAINS == 2 && !g.two) {
+                if (!g.two) {
                     // alternate key tiles: K0 K1 | V0 K2 | V1 K3 | ...
                     for (int j = 0; j < min(2, g.tiles) && ok; j++) {
                         wait_load(n_use);
@@ -499,7 +504,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         wait_load(n_use);
                         wait_p(t);
                         if (!ok) break;
-                        values(t, n_use);
+                        values(t, n_use, !F32ACT && j >= 2);
                         release(n_use++);
                         if (j + 2 < g.tiles) {
                             wait_load(n_use);
@@ -515,10 +520,8 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                     if (!ok) break;
                     scores(0, 0, n_use);
                     ptx::mma_commit(&bar.s_full[0]);
-                    if (g.two) {
-                        scores(1, 1, n_use);
-                        ptx::mma_commit(&bar.s_full[1]);
-                    }
+                    scores(1, 1, n_use);
+                    ptx::mma_commit(&bar.s_full[1]);
                     release(n_use++);
                     for (int j = 0; j < g.tiles && ok; j++) {
                         const int v = n_use, k = n_use + 1;
@@ -526,26 +529,22 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         wait_load(v);
                         wait_p(0);
                         if (!ok) break;
-                        values(0, v);
-                        if (!g.two) release(v);
+                        values(0, v, j > 0);
                         if (more) {
                             wait_load(k);
                             if (!ok) break;
                             scores(0, 0, k);
-                            if (!g.two) release(k);
                         }
                         ptx::mma_commit(&bar.s_full[0]);
-                        if (g.two) {
-                            wait_p(1);
-                            if (!ok) break;
-                            values(1, v);
-                            release(v);
-                            if (more) {
-                                scores(1, 1, k);
-                                release(k);
-                            }
-                            ptx::mma_commit(&bar.s_full[1]);
+                        wait_p(1);
+                        if (!ok) break;
+                        values(1, v, j > 0);
+                        release(v);
+                        if (more) {
+                            scores(1, 1, k);
+                            release(k);
                         }
+                        ptx::mma_commit(&bar.s_full[1]);
                         n_use += more ? 2 : 1;
                     }
                 }
@@ -558,87 +557,85 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
         }
         __syncwarp();
     } else {
-        // ------------------------------------------------ softmax, a thread per row
+        // ------------------------------------------------ softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFT));
-        const int chain = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const int wg = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // TMEM lane `row` is this thread's
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const uint32_t s_at = tmem + lanes + T::COL_S + chain * 128, o_at = tmem + lanes + T::COL_O + chain * 128;
-        const float base = p.a.scale * 1.4426950408889634f;
-        int n_s = 0, n_join = 0, tile_base = 0;
+        const float base = p.a.scale * 1.4426950408889634f;   // scores in log2 units
+        float* qs = reinterpret_cast<float*>(smem + T::OFF_QS);
+        int n_s[2] = {0, 0}, n_join = 0, n_half = 0, tile_base = 0;
         bool ok = true, was_two = false;
-        auto wait_s = [&]() {
-            ok = wait_warp(&bar.s_full[chain], n_s++ & 1, abort_flag, p.err, ERR_P_SOFT);
+        auto wait_s = [&](int t) {
+            ok = wait_warp(&bar.s_full[t], n_s[t]++ & 1, abort_flag, p.err, ERR_P_SOFT);
             ptx::tc_fence_after();
         };
-        auto meet = [&]() {   // both chains' softmax threads
+        auto meet = [&]() {   // all softmax threads
             ptx::mbar_arrive(&bar.join);
             ok = wait_warp(&bar.join, n_join++ & 1, abort_flag, p.err, ERR_P_SOFT);
+        };
+        // What comes with a tile's V (its scales, the positions taken out of it) is there once
+        // V has landed, which its product waits for, not the scores.  (Not the ring slot's
+        // barrier, which may be two phases away here: up to two later V tiles may have landed
+        // too, hence four barriers.)
+        auto wait_v = [&](int tile_no) {
+            ok = wait_warp(&bar.v_notes[tile_no & 3], (tile_no >> 2) & 1, abort_flag, p.err, ERR_P_SOFT);
         };
         while (ok && u < u_end) {
             const Segment g = segment_of<T>(p, cur, u, u_end);
             const PagedSeq& s = cur.s;
-            const bool split_keys = T::CHAINS == 2 && !g.two;
-            const int my_row = g.row0 + row + (g.two ? chain * 128 : 0);
-            const bool live = my_row < g.row0 + g.rows && (T::CHAINS == 2 || chain == 0);
+            const bool split_keys = !F32ACT && !g.two;
             if (split_keys && was_two) {   // chain 1's products have read its own Q, whose place is used below
                 meet();
                 if (!ok) break;
             }
             was_two = g.two;
-            // ---- the rows of Q into shared memory ----
-            float c_row = base;
-            uint8_t* q1 = smem + T::QP * T::PLANE;   // free when both chains share their rows
-            if (chain == 0 || g.two) {
-                const uint32_t dst = ptx::smem_u32(smem) + (uint32_t)(g.two ? chain : 0) * T::QP * T::PLANE;
-                const int64_t at = live ? (int64_t)(s.first + my_row / p.group) * p.a.q_stride[0] +
-                                              (cur.h * p.group + my_row % p.group) * p.a.q_stride[1] : 0;
+            // ---- Q into shared memory: LQ lanes a row, 8 features each ----
+            if (F32ACT || wg == 0 || g.two) {
+                constexpr int LQ = D / 8, STEP = (F32ACT ? 256 : 128) / LQ;
+                const int q_tile = g.two ? wg : 0, first = q_tile * 128, n = min(128, g.rows - first);
+                const uint32_t dst = ptx::smem_u32(smem) + (uint32_t)q_tile * T::QP * T::PLANE;
+                const int t = F32ACT ? tid - 256 : row, d = t % LQ * 8;
                 const bool bf = p.a.dtype == RT_BF16;
-                const float* qf = static_cast<const float*>(p.a.q) + at;
-                const __nv_bfloat16* qh = static_cast<const __nv_bfloat16*>(p.a.q) + at;
-                auto get8 = [&](int d, float (&x)[8]) {
-                    if (!live) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = 0.0f;
-                    } else if (bf && vec_q) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(qh + d);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            x[2 * i] = __uint_as_float(w[i] << 16);
-                            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-                        }
-                    } else if (vec_q) {
-                        const float4 a = *reinterpret_cast<const float4*>(qf + d), b = *reinterpret_cast<const float4*>(qf + d + 4);
-                        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-                        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = bf ? __bfloat162float(qh[d + i]) : qf[d + i];
-                    }
-                };
-                float up = 1.0f;
-                if constexpr (!T::DIRECT) {
-                    float m = 0.0f;
 #pragma unroll 4
-                    for (int d = 0; d < D; d += 8) {
-                        float x[8];
-                        get8(d, x);
+                for (int r = t / LQ; r < n; r += STEP) {   // (rows past the item hold whatever was there: their results go nowhere)
+                    const int rr = g.row0 + first + r;
+                    const int64_t at = (int64_t)(s.first + rr / p.group) * p.a.q_stride[0] + (cur.h * p.group + rr % p.group) * p.a.q_stride[1] + d;
+                    const float* qf = static_cast<const float*>(p.a.q) + at;
+                    const __nv_bfloat16* qh = static_cast<const __nv_bfloat16*>(p.a.q) + at;
+                    const uint32_t a = dst + tile_at(r, d * 2);
+                    if constexpr (T::DIRECT) {
+                        if (vec_q) {
+                            cp_async16(a, qh, true);
+                        } else {
+                            const unsigned short* q16 = reinterpret_cast<const unsigned short*>(qh);
+                            st_shared16(a, q16[0] | q16[1] << 16, q16[2] | q16[3] << 16, q16[4] | q16[5] << 16, q16[6] | q16[7] << 16);
+                        }
+                    } else {
+                        float x[8], h[8], m = 0.0f;
+                        if (bf && vec_q) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(qh);
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                x[2 * i] = __uint_as_float(w[i] << 16);
+                                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                            }
+                        } else if (vec_q) {
+                            const float4 v = *reinterpret_cast<const float4*>(qf), w = *reinterpret_cast<const float4*>(qf + 4);
+                            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+                            x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) x[i] = bf ? __bfloat162float(qh[i]) : qf[i];
+                        }
 #pragma unroll
                         for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
-                    }
-                    const int e = f16_scale_exp(m);
-                    up = pow2i(e);
-                    c_row = base * pow2i(-e);
-                }
-#pragma unroll 4
-                for (int d = 0; d < D; d += 8) {
-                    float x[8];
-                    get8(d, x);
-                    const uint32_t a = dst + tile_at(row, d * 2);
-                    if constexpr (T::DIRECT) {
-                        st_shared16(a, bf16_pair_rn(x[0], x[1]), bf16_pair_rn(x[2], x[3]), bf16_pair_rn(x[4], x[5]), bf16_pair_rn(x[6], x[7]));
-                    } else {
-                        float h[8];
+                        const uint32_t mates = (LQ == 16 ? 0xffffu : 0xffu) << (lane / LQ * LQ);
+#pragma unroll
+                        for (int i = LQ / 2; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(mates, m, i));
+                        const int e = f16_scale_exp(m);
+                        const float up = pow2i(e);
+                        if (t % LQ == 0) qs[first + r] = base * pow2i(-e);
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             x[i] *= up;
@@ -650,158 +647,245 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                                         f16x2_rn(x[4] - h[4], x[5] - h[5]), f16x2_rn(x[6] - h[6], x[7] - h[7]));
                     }
                 }
-                if (split_keys && !T::DIRECT) reinterpret_cast<float*>(q1)[row] = c_row;
+                if constexpr (T::DIRECT) {
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    cp_wait<0>();
+                }
                 ptx::fence_proxy_async_smem();
-                if (T::CHAINS == 2 || chain == 0) ptx::mbar_arrive(&bar.q_full[g.two ? chain : 0]);
+                ptx::mbar_arrive(&bar.q_full[q_tile]);
             }
-            // ---- tiles ----
+            // ---- this thread's row ----
+            const int my_row = g.row0 + row + (g.two ? wg * 128 : 0);
+            const bool live = my_row < g.row0 + g.rows, any_live = __any_sync(0xffffffffu, live);
             const int at_pos = s.L - s.n + my_row / p.group;
             const int lo_row = p.a.window > 0 ? max(0, at_pos - p.a.window + 1) : 0;
             const int hi_row = live ? (p.a.causal ? min(s.L, at_pos + 1) : s.L) : 0;
-            const bool any_live = __any_sync(0xffffffffu, live);
-            float m = -INFINITY, l = 0.0f, ref = 0.0f, v_top = 0.0f;   // ref: what exponents are taken against
-            float o[D];
+            float c_row = base, m = -INFINITY, l = 0.0f, ref = 0.0f, v_top = 0.0f;   // ref: what exponents are taken against
+            // Scores of N positions from b on: times their scales, -inf where the row does not see them; their maximum.
+            auto see = [&](auto& x, int b, int tile_no, int k0, bool masked) -> float {
+                constexpr int N = sizeof(x) / 4;
+                if constexpr (!T::DIRECT) {
+                    const float* ks = reinterpret_cast<const float*>(smem + T::OFF_KS) + tile_no % T::KSD * 128 + b;
 #pragma unroll
-            for (int i = 0; i < D; i++) o[i] = 0.0f;
-            auto fold = [&]() {
+                    for (int i = 0; i < N; i += 4) {
+                        const float4 k = *reinterpret_cast<const float4*>(ks + i);
+                        upk2(mul2(pk2(x[i], x[i + 1]), pk2(k.x, k.y)), x[i], x[i + 1]);
+                        upk2(mul2(pk2(x[i + 2], x[i + 3]), pk2(k.z, k.w)), x[i + 2], x[i + 3]);
+                    }
+                }
+                if (masked) {
 #pragma unroll
-                for (int b = 0; b < D; b += 16) {
-                    uint32_t r[16];
-                    ptx::tmem_ld16(o_at + b, r);
-                    ptx::tmem_ld_wait();
+                    for (int w = 0; w < N / 32; w++) {
+                        const uint32_t there = bar.ok[tile_no & 7][(b >> 5) + w];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-                        upk2(add2(pk2(o[b + i], o[b + i + 1]), pk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]))), o[b + i], o[b + i + 1]);
+                        for (int i = 0; i < 32; i++) {
+                            const int k = k0 + b + w * 32 + i;
+                            if (!((there >> i & 1) && k >= lo_row && k < hi_row)) x[w * 32 + i] = -INFINITY;
+                        }
+                    }
+                }
+                float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    t0 = max3f(t0, x[i], x[i + 1]);
+                    t1 = max3f(t1, x[i + 2], x[i + 3]);
+                }
+                return fmaxf(t0, t1) * c_row;
+            };
+            auto sees_all = [&](int k0, int tile_no) {
+                const uint32_t* w = bar.ok[tile_no & 7];
+                return lo_row <= k0 && hi_row >= k0 + TKT && (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu;
+            };
+            // Moves the reference when a score or a value scale asks for it; the factor for what
+            // has been summed, 1 where nothing moved.
+            auto refer = [&](float top, int tile_no) -> float {
+                float tile_v = 0.0f;
+                if constexpr (!T::DIRECT) {
+                    const float* vm = bar.vmax[tile_no & 3];
+                    tile_v = fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3]));
+                }
+                const bool raise = top > m + RAISE, wider = !T::DIRECT && tile_v > v_top;
+                if (!raise && !wider) return 1.0f;
+                if (raise) m = top;
+                if (wider) v_top = 4.0f * tile_v;
+                const float to = (m == -INFINITY ? 0.0f : m) + (T::DIRECT ? 0.0f : fmaxf(log2f(v_top), -100.0f) - W_LOG2);
+                const float f = l == 0.0f ? 0.0f : exp2_fast(ref - to);   // (nothing summed yet: o = 0)
+                ref = to;
+                l *= f;
+                return f;
+            };
+            // Scores to weights, in place; their sum.  Then times the value scales.
+            auto weigh = [&](auto& x, int b, int tile_no, bool masked) {
+                constexpr int N = sizeof(x) / 4;
+                const unsigned long long cc = pk2(c_row, c_row), nr = pk2(-ref, -ref);
+                unsigned long long s0 = pk2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    upk2(fma2(pk2(x[i], x[i + 1]), cc, nr), x[i], x[i + 1]);
+                    upk2(fma2(pk2(x[i + 2], x[i + 3]), cc, nr), x[i + 2], x[i + 3]);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) x[i + k] = exp2_fast(x[i + k]);
+                    s0 = add2(s0, pk2(x[i], x[i + 1]));
+                    s1 = add2(s1, pk2(x[i + 2], x[i + 3]));
+                }
+                float a, c2;
+                upk2(add2(s0, s1), a, c2);
+                l += a + c2;
+                if constexpr (!T::DIRECT) {
+                    const float* vs = reinterpret_cast<const float*>(smem + T::OFF_VS) + tile_no % T::VSD * 128 + b;
+#pragma unroll
+                    for (int i = 0; i < N; i += 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(vs + i);
+                        const float w[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
+                        upk2(mul2(pk2(x[i], x[i + 1]), pk2(v.x, v.y)), x[i], x[i + 1]);
+                        upk2(mul2(pk2(x[i + 2], x[i + 3]), pk2(v.z, v.w)), x[i + 2], x[i + 3]);
+                        if (masked) {   // a position that is not seen may have any scale
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                if (w[k] == 0.0f) x[i + k] = 0.0f;
+                        }
+                    }
                 }
             };
-            const int step = split_keys ? 2 : 1, j0 = split_keys ? chain : 0;
-            const bool works = T::CHAINS == 2 ? (split_keys || g.two || chain == 0) : chain == 0;
-            if (works && j0 < g.tiles) {
-                for (int j = j0; j < g.tiles; j += step) {
-                    const int tile_no = tile_base + j, k0 = g.k0 + j * TKT;
-                    wait_s();
+            constexpr int NO = F32ACT ? D / 2 : D;   // this thread's output columns
+            const int col0 = F32ACT ? wg * (D / 2) : 0;
+            float o[NO];
+            if constexpr (F32ACT) {
+                // Two threads a row, 64 positions and D / 2 output columns each; S, P and O of even
+                // and odd tiles in places of their own.  A tile's O is folded into registers two
+                // tiles later, when its scores' successors are ready.
+                float* red = reinterpret_cast<float*>(smem + T::OFF_RED);
+                float ref_of[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < NO; i++) o[i] = 0.0f;
+                auto fold = [&](int t) {
+                    const float f = ref_of[t] == ref ? 1.0f : exp2_fast(ref_of[t] - ref);
+                    const unsigned long long ff = pk2(f, f);
+#pragma unroll
+                    for (int b = 0; b < NO; b += 32) {
+                        uint32_t r[32];
+                        ptx::tmem_ld32(tmem + lanes + T::COL_O + t * 128 + col0 + b, r);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2)
+                            upk2(fma2(pk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), ff, pk2(o[b + i], o[b + i + 1])), o[b + i], o[b + i + 1]);
+                    }
+                };
+                for (int j = 0; j < g.tiles; j++) {
+                    const int t = j & 1, tile_no = tile_base + j, k0 = g.k0 + j * TKT;
+                    wait_s(t);
                     if (!ok) break;
-                    if (j == j0 && split_keys && chain == 1 && !T::DIRECT) c_row = reinterpret_cast<const float*>(q1)[row];
-                    // What comes with V_j (its scales, the positions taken out of it) is there once
-                    // V_j has landed, which its product waits for, not the scores.  (Not the ring
-                    // slot's barrier, which may be two phases away here: up to two later V
-                    // tiles may have landed too, hence four barriers.)
-                    auto wait_v = [&]() {
-                        ok = wait_warp(&bar.v_notes[tile_no & 3], (tile_no >> 2) & 1, abort_flag, p.err, ERR_P_SOFT);
-                    };
+                    if (j == 0) c_row = qs[row];
                     if (any_live) {
-                        const float* ks = reinterpret_cast<const float*>(smem + T::OFF_KS) + tile_no % (T::DIRECT ? 1 : T::KSD) * 128;
-                        const float* vs = reinterpret_cast<const float*>(smem + T::OFF_VS) + tile_no % (T::DIRECT ? 1 : T::VSD) * 128;
-                        const uint32_t* okw = bar.ok[tile_no & 7];
-                        const bool whole = lo_row <= k0 && hi_row >= k0 + TKT && (okw[0] & okw[1] & okw[2] & okw[3]) == 0xffffffffu;
-                        const bool masked = __any_sync(0xffffffffu, live && !whole);
-                        // the largest score
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int b = 0; b < TKT; b += 16) {
-                            uint32_t r[16];
-                            ptx::tmem_ld16(s_at + b, r);
+                        const uint32_t s_at = tmem + lanes + T::COL_S + t * 128 + wg * 64;
+                        const bool masked = __any_sync(0xffffffffu, live && !sees_all(k0, tile_no));
+                        float x[64];
+                        {
+                            uint32_t(&r)[64] = reinterpret_cast<uint32_t(&)[64]>(x);
+                            ptx::tmem_ld32(s_at, reinterpret_cast<uint32_t(&)[32]>(r[0]));
+                            ptx::tmem_ld32(s_at + 32, reinterpret_cast<uint32_t(&)[32]>(r[32]));
                             ptx::tmem_ld_wait();
-                            float x[16];
-#pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = __uint_as_float(r[i]);
-                            if constexpr (!T::DIRECT) {
-#pragma unroll
-                                for (int i = 0; i < 16; i += 4) {
-                                    const float4 k = *reinterpret_cast<const float4*>(ks + b + i);
-                                    x[i] *= k.x; x[i + 1] *= k.y; x[i + 2] *= k.z; x[i + 3] *= k.w;
-                                }
-                            }
-                            if (masked) {
-                                const uint32_t w = okw[b >> 5] >> (b & 16);
-#pragma unroll
-                                for (int i = 0; i < 16; i++)
-                                    if (!((w >> i & 1) && k0 + b + i >= lo_row && k0 + b + i < hi_row)) x[i] = -INFINITY;
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) top = max3f(top, x[i], x[i + 1]);
                         }
-                        top *= c_row;
-                        if (j > j0) fold();
-                        if (!T::DIRECT || masked) {
-                            wait_v();
-                            if (!ok) break;
-                        }
-                        // the reference
-                        float tile_v = 1.0f;
-                        if constexpr (!T::DIRECT) {
-                            const float* vm = bar.vmax[tile_no & 3];
-                            tile_v = fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3]));
-                        }
-                        const bool raise = top > m + RAISE, wider = !T::DIRECT && tile_v > v_top;
-                        if (raise) m = top;
-                        if (wider) v_top = 4.0f * tile_v;
-                        if (__any_sync(0xffffffffu, raise || wider)) {
-                            const float to = (m == -INFINITY ? 0.0f : m) + (T::DIRECT ? 0.0f : fmaxf(log2f(v_top), -100.0f) - W_LOG2);
-                            const float f = l == 0.0f ? 0.0f : exp2_fast(ref - to);   // (nothing summed yet: o = 0)
-                            ref = to;
-                            l *= f;
+                        float top = see(x, wg * 64, tile_no, k0, masked);
+                        // the row's other half: read for tile j - 2 before anyone got here
+                        red[(t * 2 + wg) * 128 + row] = top;
+                        ptx::mbar_arrive(&bar.half[quarter]);
+                        ok = wait_warp(&bar.half[quarter], n_half++ & 1, abort_flag, p.err, ERR_P_SOFT);
+                        if (!ok) break;
+                        top = fmaxf(top, red[(t * 2 + (wg ^ 1)) * 128 + row]);
+                        wait_v(tile_no);
+                        if (!ok) break;
+                        const float f = refer(top, tile_no);
+                        if (__any_sync(0xffffffffu, f != 1.0f)) {
                             const unsigned long long ff = pk2(f, f);
 #pragma unroll
-                            for (int i = 0; i < D; i += 2) upk2(mul2(pk2(o[i], o[i + 1]), ff), o[i], o[i + 1]);
+                            for (int i = 0; i < NO; i += 2) upk2(mul2(pk2(o[i], o[i + 1]), ff), o[i], o[i + 1]);
                         }
-                        // weights
-                        unsigned long long sum = pk2(0.0f, 0.0f);
-                        const unsigned long long cc = pk2(c_row, c_row), nr = pk2(-ref, -ref);
+                        if (j >= 2) fold(t);
+                        ref_of[t] = ref;
+                        weigh(x, wg * 64, tile_no, masked);
 #pragma unroll
-                        for (int b = 0; b < TKT; b += 16) {
-                            uint32_t r[16];
-                            ptx::tmem_ld16(s_at + b, r);
+                        for (int b = 0; b < 64; b += 16) {   // per 16 positions: 8 columns of hi pairs, 8 of lo pairs
+                            uint32_t w[16];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                const float ha = __uint_as_float(__float_as_uint(x[b + 2 * i]) & 0xffffe000u);
+                                const float hb = __uint_as_float(__float_as_uint(x[b + 2 * i + 1]) & 0xffffe000u);
+                                w[i] = f16x2_rn(ha, hb);
+                                w[8 + i] = f16x2_rn(x[b + 2 * i] - ha, x[b + 2 * i + 1] - hb);
+                            }
+                            ptx::tmem_st16(s_at + b, w);
+                        }
+                        ptx::tmem_st_wait();
+                    }
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(&bar.p_full[t]);
+                }
+                for (int j = max(0, g.tiles - 2); ok && j < g.tiles; j++) {
+                    wait_s(j & 1);
+                    if (ok && any_live) fold(j & 1);
+                }
+                if (!ok) break;
+                ptx::tc_fence_before();
+                if (any_live) {   // the weight sum of both halves
+                    const int t = g.tiles & 1;
+                    red[(t * 2 + wg) * 128 + row] = l;
+                    ptx::mbar_arrive(&bar.half[quarter]);
+                    ok = wait_warp(&bar.half[quarter], n_half++ & 1, abort_flag, p.err, ERR_P_SOFT);
+                    if (!ok) break;
+                    l = wg ? red[t * 2 * 128 + row] + l : l + red[(t * 2 + 1) * 128 + row];
+                }
+            } else {
+                // A thread per row; O stays in TMEM and is rescaled there when the reference moves.
+                const int chain = wg, step = split_keys ? 2 : 1;
+                const uint32_t s_at = tmem + lanes + T::COL_S + chain * 128, o_at = tmem + lanes + T::COL_O + chain * 128;
+                const int j0 = split_keys ? chain : 0;
+                for (int j = j0; j < g.tiles; j += step) {
+                    const int tile_no = tile_base + j, k0 = g.k0 + j * TKT;
+                    wait_s(chain);
+                    if (!ok) break;
+                    if (!T::DIRECT && j == j0) c_row = qs[row + (g.two ? chain * 128 : 0)];
+                    if (any_live) {
+                        const bool masked = __any_sync(0xffffffffu, live && !sees_all(k0, tile_no));
+                        float x[128];
+                        {
+                            uint32_t(&r)[128] = reinterpret_cast<uint32_t(&)[128]>(x);
+#pragma unroll
+                            for (int b = 0; b < 128; b += 32) ptx::tmem_ld32(s_at + b, reinterpret_cast<uint32_t(&)[32]>(r[b]));
                             ptx::tmem_ld_wait();
-                            float x[16];
+                        }
+                        const float top = see(x, 0, tile_no, k0, masked);
+                        if (!T::DIRECT || masked) {
+                            wait_v(tile_no);
+                            if (!ok) break;
+                        }
+                        const float f = refer(top, tile_no);
+                        if (j > j0 && __any_sync(0xffffffffu, f != 1.0f)) {
+                            const unsigned long long ff = pk2(f, f);
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                unsigned long long y = pk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-                                if constexpr (!T::DIRECT) y = mul2(y, *reinterpret_cast<const unsigned long long*>(ks + b + i));
-                                upk2(fma2(y, cc, nr), x[i], x[i + 1]);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = exp2_fast(x[i]);
-                            if (masked) {
-                                const uint32_t w = okw[b >> 5] >> (b & 16);
-#pragma unroll
-                                for (int i = 0; i < 16; i++)
-                                    if (!((w >> i & 1) && k0 + b + i >= lo_row && k0 + b + i < hi_row)) x[i] = 0.0f;
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) sum = add2(sum, pk2(x[i], x[i + 1]));
-                            if constexpr (!T::DIRECT) {
+                            for (int b = 0; b < D; b += 16) {
+                                uint32_t r[16];
+                                ptx::tmem_ld16(o_at + b, r);
+                                ptx::tmem_ld_wait();
 #pragma unroll
                                 for (int i = 0; i < 16; i += 2) {
-                                    const bool z0 = masked && x[i] == 0.0f, z1 = masked && x[i + 1] == 0.0f;
-                                    upk2(mul2(pk2(x[i], x[i + 1]), *reinterpret_cast<const unsigned long long*>(vs + b + i)), x[i], x[i + 1]);
-                                    if (z0) x[i] = 0.0f;   // a position that is not seen may have any scale
-                                    if (z1) x[i + 1] = 0.0f;
+                                    float a, c2;
+                                    upk2(mul2(pk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), ff), a, c2);
+                                    r[i] = __float_as_uint(a);
+                                    r[i + 1] = __float_as_uint(c2);
                                 }
+                                ptx::tmem_st16(o_at + b, r);
                             }
-                            uint32_t hi[8];
-                            if constexpr (T::DIRECT) {
-#pragma unroll
-                                for (int i = 0; i < 8; i++) hi[i] = bf16_pair_rn(x[2 * i], x[2 * i + 1]);
-                            } else if constexpr (T::QP == 1) {
-#pragma unroll
-                                for (int i = 0; i < 8; i++) hi[i] = f16x2_rn(x[2 * i], x[2 * i + 1]);
-                            } else {
-                                uint32_t lo[8];
-#pragma unroll
-                                for (int i = 0; i < 8; i++) {
-                                    const float a = __uint_as_float(__float_as_uint(x[2 * i]) & 0xffffe000u);
-                                    const float d = __uint_as_float(__float_as_uint(x[2 * i + 1]) & 0xffffe000u);
-                                    hi[i] = f16x2_rn(a, d);
-                                    lo[i] = f16x2_rn(x[2 * i] - a, x[2 * i + 1] - d);
-                                }
-                                ptx::tmem_st8(s_at + b + 8, lo);
-                            }
-                            ptx::tmem_st8(s_at + b, hi);
                         }
-                        float s0, s1;
-                        upk2(sum, s0, s1);
-                        l += s0 + s1;
+                        weigh(x, 0, tile_no, masked);
+#pragma unroll
+                        for (int b = 0; b < 128; b += 32) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                w[i] = T::DIRECT ? bf16_pair_rn(x[b + 2 * i], x[b + 2 * i + 1]) : f16x2_rn(x[b + 2 * i], x[b + 2 * i + 1]);
+                            ptx::tmem_st16(s_at + b / 2, w);
+                        }
                         if constexpr (T::DIRECT) {
                             if (masked) {   // values that are not finite were taken out: rows that see one get NaN
                                 const uint32_t* sw = bar.strange[tile_no & 7];
@@ -815,82 +899,93 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                     ptx::tc_fence_before();
                     ptx::mbar_arrive(&bar.p_full[chain]);
                 }
-                if (ok) wait_s();
-                if (!ok) break;
-                if (any_live) fold();
-                ptx::tc_fence_before();
-            }
-            // ---- the other chain's share of the keys ----
-            if (split_keys) {
-                float* x = reinterpret_cast<float*>(q1);
-                if (chain == 1) {
-                    x[row] = l == 0.0f ? -INFINITY : ref;
-                    x[128 + row] = l;
-                }
-                meet();
-                if (!ok) break;
-                float f0 = 1.0f, f1 = 0.0f;
-                if (chain == 0) {
-                    const float r1 = x[row], l1 = x[128 + row];
-                    const float r0 = l == 0.0f ? -INFINITY : ref, to = fmaxf(r0, r1);
-                    if (to != -INFINITY) {
-                        f0 = l == 0.0f ? 0.0f : exp2_fast(r0 - to);
-                        f1 = l1 == 0.0f ? 0.0f : exp2_fast(r1 - to);
-                        l = l * f0 + l1 * f1;
-                        ref = to;
-                    }
-                }
-                meet();
                 if (!ok) break;
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
+                for (int i = 0; i < NO; i++) o[i] = 0.0f;
+                if (j0 < g.tiles) {
+                    wait_s(chain);
+                    if (!ok) break;
+                    if (any_live) {
+                        uint32_t(&r)[NO] = reinterpret_cast<uint32_t(&)[NO]>(o);
+#pragma unroll
+                        for (int b = 0; b < D; b += 32) ptx::tmem_ld32(o_at + b, reinterpret_cast<uint32_t(&)[32]>(r[b]));
+                        ptx::tmem_ld_wait();
+                    }
+                    ptx::tc_fence_before();
+                }
+                if (split_keys) {   // the other chain's share of the keys
+                    float* x = reinterpret_cast<float*>(smem + T::QP * T::PLANE);   // the second Q tile's place
                     if (chain == 1) {
-#pragma unroll
-                        for (int i = 0; i < D / 2; i++) x[i * 128 + row] = o[half * (D / 2) + i];
+                        x[row] = l == 0.0f ? -INFINITY : ref;
+                        x[128 + row] = l;
                     }
                     meet();
                     if (!ok) break;
+                    float f0 = 1.0f, f1 = 0.0f;
                     if (chain == 0) {
-#pragma unroll
-                        for (int i = 0; i < D / 2; i++) o[half * (D / 2) + i] = o[half * (D / 2) + i] * f0 + x[i * 128 + row] * f1;
+                        const float r1 = x[row], l1 = x[128 + row];
+                        const float r0 = l == 0.0f ? -INFINITY : ref, to = fmaxf(r0, r1);
+                        if (to != -INFINITY) {
+                            f0 = l == 0.0f ? 0.0f : exp2_fast(r0 - to);
+                            f1 = l1 == 0.0f ? 0.0f : exp2_fast(r1 - to);
+                            l = l * f0 + l1 * f1;
+                            ref = to;
+                        }
                     }
                     meet();
+                    if (!ok) break;
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        if (chain == 1) {
+#pragma unroll
+                            for (int i = 0; i < D / 2; i++) x[i * 128 + row] = o[half * (D / 2) + i];
+                        }
+                        meet();
+                        if (!ok) break;
+                        if (chain == 0) {
+#pragma unroll
+                            for (int i = 0; i < D / 2; i++) o[half * (D / 2) + i] = o[half * (D / 2) + i] * f0 + x[i * 128 + row] * f1;
+                        }
+                        meet();
+                        if (!ok) break;
+                    }
                     if (!ok) break;
                 }
-                if (!ok) break;
             }
             // ---- out ----
-            if (live && (chain == 0 || g.two)) {
+            if (live && (F32ACT || wg == 0 || g.two)) {
                 if (cur.i == 0 && g.tiles == cur.t.count) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const int64_t at = paged_out_at(p, s, cur.h, my_row);
+                    const int64_t at = paged_out_at(p, s, cur.h, my_row) + col0;
                     if (!vec_out) {
 #pragma unroll
-                        for (int i = 0; i < D; i++) {
+                        for (int i = 0; i < NO; i++) {
                             if (p.a.dtype == RT_BF16) static_cast<__nv_bfloat16*>(p.a.out)[at + i] = __float2bfloat16_rn(o[i] * inv);
                             else static_cast<float*>(p.a.out)[at + i] = o[i] * inv;
                         }
                     } else if (p.a.dtype == RT_BF16) {
                         uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + at);
 #pragma unroll
-                        for (int i = 0; i < D / 8; i++)
+                        for (int i = 0; i < NO / 8; i++)
                             out[i] = make_uint4(bf16_pair_rn(o[8 * i] * inv, o[8 * i + 1] * inv), bf16_pair_rn(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                                                 bf16_pair_rn(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16_pair_rn(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
                     } else {
                         float4* out = reinterpret_cast<float4*>(static_cast<float*>(p.a.out) + at);
 #pragma unroll
-                        for (int i = 0; i < D / 4; i++)
+                        for (int i = 0; i < NO / 4; i++)
                             out[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
                     }
-                    paged_store_lse(p, s, cur.h, my_row, ref, l);
+                    if (col0 == 0) paged_store_lse(p, s, cur.h, my_row, ref, l);
                 } else {
                     float* part = p.part + (int64_t)(2 * blockIdx.x + (cur.i == 0)) * T::OUT;
                     const int r = my_row - g.row0;
-                    float4* out = reinterpret_cast<float4*>(part + r * D);
+                    float4* out = reinterpret_cast<float4*>(part + r * D + col0);
 #pragma unroll
-                    for (int i = 0; i < D / 4; i++) out[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    part[T::R * D + r] = l == 0.0f ? -INFINITY : ref;
-                    part[T::R * D + T::R + r] = l;
+                    for (int i = 0; i < NO / 4; i++) out[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    if (col0 == 0) {
+                        part[T::R * D + r] = l == 0.0f ? -INFINITY : ref;
+                        part[T::R * D + T::R + r] = l;
+                    }
                 }
             }
             tile_base += g.tiles;
@@ -907,9 +1002,11 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
 
 constexpr int MIN_UNITS = 4;
 
+int tile_rows(const RtPagedAttention& p) { return p.cache.dtype == RT_F32 || p.dtype == RT_F32 ? 128 : 256; }
+
 // Blocks of a call: one per SM, no more than it has work for.
 int tiles_blocks(const RtPagedAttention& p) {
-    const int R = p.cache.dtype == RT_F32 ? 128 : 256;
+    const int R = tile_rows(p);
     const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(p.max_new, p.total_new)) * (p.n_q_heads / p.cache.n_heads);
     const int64_t units = (int64_t)p.n_seqs * p.cache.n_heads * ((rows + R - 1) / R) * std::max(1, (p.max_kv + TKT - 1) / TKT);
     return (int)std::max<int64_t>(1, std::min<int64_t>(g_num_sms, (units + MIN_UNITS - 1) / MIN_UNITS));
@@ -942,7 +1039,7 @@ Status tiles_dim(PagedArgs& p, void* ws, cudaStream_t st) {
 bool paged_tiles_takes(const RtPagedAttention& p) { return p.cache.head_dim == 64 || p.cache.head_dim == 128; }
 
 size_t paged_tiles_workspace(const RtPagedAttention& p) {
-    const int R = p.cache.dtype == RT_F32 ? 128 : 256;
+    const int R = tile_rows(p);
     return (size_t)tiles_blocks(p) * 2 * (R * p.cache.head_dim + 2 * R) * sizeof(float);
 }
 
