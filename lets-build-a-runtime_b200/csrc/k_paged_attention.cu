@@ -1,10 +1,12 @@
 // k_paged_attention.cu -- attention of new tokens over a paged cache: which
 // kernel takes a call.
 //
-// More than 16 rows (new tokens x query heads of a cache head) fill a tensor
-// core tile of 128 well enough to beat reading the cache once per 16 rows;
-// head dims other than 64 and 128 have no such tiles and take the few-rows
-// kernel whatever their rows.
+// The few-rows kernel takes up to 32 rows (new tokens x query heads of a cache
+// head) in one pass over the cache when its products have one part (bf16
+// activations over a bf16 or 8-bit cache), 16 otherwise; more rows fill a tensor
+// core tile of 128 well enough to beat reading the cache once per 16 or 32.
+// Head dims other than 64 and 128 have no such tiles and take the few-rows kernel
+// whatever their rows.
 #include "paged.h"
 
 namespace rt {
@@ -12,7 +14,7 @@ namespace {
 
 bool use_tiles(const RtPagedAttention& p) {
     const int64_t rows = (int64_t)(p.max_new < p.total_new ? p.max_new : p.total_new) * (p.n_q_heads / p.cache.n_heads);
-    return rows > 16 && paged_tiles_takes(p);
+    return rows > (p.dtype == RT_BF16 && p.cache.dtype != RT_F32 ? 32 : 16) && paged_tiles_takes(p);
 }
 
 }  // namespace
@@ -26,6 +28,8 @@ Status launch_paged_attention(const RtPagedAttention& a, void* ws, cudaStream_t 
     p.a = a;
     p.err = kernel_error_flag();
     p.group = a.n_q_heads / a.cache.n_heads;
+    p.vec_q = paged_rows16(a.q, a.q_stride, a.dtype);
+    p.vec_out = paged_rows16(a.out, a.out_stride, a.dtype);
     p.page_shift = -1;
     for (int i = 0; i < 31; i++)
         if (a.cache.page_size == 1 << i) p.page_shift = i;

@@ -184,7 +184,7 @@ __device__ __forceinline__ Segment segment_of(const PagedArgs& p, const PagedCur
 }
 
 template <int CT, bool F32ACT, int D>
-__global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constant__ PagedArgs p, const bool vec_q, const bool vec_out) {
+__global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constant__ PagedArgs p) {
     using T = Tile<CT, F32ACT, D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bar = *reinterpret_cast<Bars*>(smem + T::OFF_BAR);
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                     const __nv_bfloat16* qh = static_cast<const __nv_bfloat16*>(p.a.q) + at;
                     const uint32_t a = dst + tile_at(r, d * 2);
                     if constexpr (T::DIRECT) {
-                        if (vec_q) {
+                        if (p.vec_q) {
                             cp_async16(a, qh, true);
                         } else {
                             const unsigned short* q16 = reinterpret_cast<const unsigned short*>(qh);
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         }
                     } else {
                         float x[8], h[8], m = 0.0f;
-                        if (bf && vec_q) {
+                        if (bf && p.vec_q) {
                             const uint4 v = *reinterpret_cast<const uint4*>(qh);
                             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                                 x[2 * i] = __uint_as_float(w[i] << 16);
                                 x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
                             }
-                        } else if (vec_q) {
+                        } else if (p.vec_q) {
                             const float4 v = *reinterpret_cast<const float4*>(qf), w = *reinterpret_cast<const float4*>(qf + 4);
                             x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
                             x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
@@ -957,7 +957,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 if (cur.i == 0 && g.tiles == cur.t.count) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                     const int64_t at = paged_out_at(p, s, cur.h, my_row) + col0;
-                    if (!vec_out) {
+                    if (!p.vec_out) {
 #pragma unroll
                         for (int i = 0; i < NO; i++) {
                             if (p.a.dtype == RT_BF16) static_cast<__nv_bfloat16*>(p.a.out)[at + i] = __float2bfloat16_rn(o[i] * inv);
@@ -1012,10 +1012,6 @@ int tiles_blocks(const RtPagedAttention& p) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(g_num_sms, (units + MIN_UNITS - 1) / MIN_UNITS));
 }
 
-bool rows16(const void* p, const int64_t st[2], int dtype) {
-    return aligned16(p) && (st[0] * dtype_bytes(dtype)) % 16 == 0 && (st[1] * dtype_bytes(dtype)) % 16 == 0;
-}
-
 template <int CT, bool F32ACT, int D>
 Status tiles_as(PagedArgs& p, void* ws, cudaStream_t st) {
     using T = Tile<CT, F32ACT, D>;
@@ -1025,7 +1021,7 @@ Status tiles_as(PagedArgs& p, void* ws, cudaStream_t st) {
     p.part = static_cast<float*>(ws);
     p.whole = 0;
     p.min_units = MIN_UNITS;
-    paged_tiles_kernel<CT, F32ACT, D><<<blocks, TT, T::SMEM, st>>>(p, rows16(p.a.q, p.a.q_stride, p.a.dtype), rows16(p.a.out, p.a.out_stride, p.a.dtype));
+    paged_tiles_kernel<CT, F32ACT, D><<<blocks, TT, T::SMEM, st>>>(p);
     RT_LAUNCH_CHECK();
     return blocks == 1 ? Status::ok() : launch_paged_join<D, T::R, TKT>(p, blocks, st);
 }

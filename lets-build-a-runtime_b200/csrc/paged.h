@@ -27,7 +27,11 @@ struct PagedArgs {
     int whole;         // 1: a block takes whole items (no join)
     int min_units;
     int page_shift;    // log2 of the page size, -1 when it is not a power of two
+    bool vec_q, vec_out;   // every row of q / out starts on 16 bytes
 };
+inline bool paged_rows16(const void* p, const int64_t st[2], int dtype) {
+    return aligned16(p) && (st[0] * dtype_bytes(dtype)) % 16 == 0 && (st[1] * dtype_bytes(dtype)) % 16 == 0;
+}
 
 struct PagedSeq {
     int b, first, n, L;   // sequence, first row of q, new tokens, cached positions
@@ -199,15 +203,36 @@ __device__ __forceinline__ float exp2_fast(float x) {   // 2^x; 2^-inf = 0
     return y;
 }
 
-// Feature d of row `row` (of the sequence's rows under cache head h), and the
-// row's log-sum-exp from its maximum (log2 units) and weight sum.
+// Where row `row` (of the sequence's rows under cache head h) goes, and its
+// log-sum-exp from its maximum (log2 units) and weight sum.
 __device__ __forceinline__ int64_t paged_out_at(const PagedArgs& p, const PagedSeq& s, int h, int row) {
     return (int64_t)(s.first + row / p.group) * p.a.out_stride[0] + (h * p.group + row % p.group) * p.a.out_stride[1];
 }
-__device__ __forceinline__ void paged_store(const PagedArgs& p, const PagedSeq& s, int h, int row, int d, float x) {
+// Four features from d on (d a multiple of 4), as one store where rows allow it.
+__device__ __forceinline__ void paged_store4(const PagedArgs& p, const PagedSeq& s, int h, int row, int d, float a, float b, float c, float e) {
     const int64_t at = paged_out_at(p, s, h, row) + d;
-    if (p.a.dtype == RT_BF16) static_cast<__nv_bfloat16*>(p.a.out)[at] = __float2bfloat16_rn(x);
-    else static_cast<float*>(p.a.out)[at] = x;
+    if (p.a.dtype == RT_BF16) {
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out) + at;
+        if (p.vec_out) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, e);
+            *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+        } else {
+            out[0] = __float2bfloat16_rn(a);
+            out[1] = __float2bfloat16_rn(b);
+            out[2] = __float2bfloat16_rn(c);
+            out[3] = __float2bfloat16_rn(e);
+        }
+    } else {
+        float* out = static_cast<float*>(p.a.out) + at;
+        if (p.vec_out) {
+            *reinterpret_cast<float4*>(out) = make_float4(a, b, c, e);
+        } else {
+            out[0] = a;
+            out[1] = b;
+            out[2] = c;
+            out[3] = e;
+        }
+    }
 }
 __device__ __forceinline__ void paged_store_lse(const PagedArgs& p, const PagedSeq& s, int h, int row, float m, float l) {
     if (p.a.lse)
@@ -250,9 +275,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
                 sum[0] += x.x * f; sum[1] += x.y * f; sum[2] += x.z * f; sum[3] += x.w * f;
                 ls += part[R * DP + R + r] * f;
             }
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (d + j < p.a.cache.head_dim) paged_store(p, s, cur.h, row0 + r, d + j, ls == 0.0f ? 0.0f : sum[j] / ls);
+        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+        if (d < p.a.cache.head_dim) paged_store4(p, s, cur.h, row0 + r, d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
         if (d == 0) paged_store_lse(p, s, cur.h, row0 + r, m, ls);
     }
 }
