@@ -7,13 +7,17 @@
 // 2^8.  With R rows sharing one pass over the keys and values the call does
 // 4 R operations per cached feature and reads it once: it is bound by HBM.
 //
-// So the work is laid out for loads in flight, not for the matrix rate: every
-// warp runs alone over blocks of 32 positions and keeps STAGES - 1 pieces of
-// 8 KB under way with cp.async.  The order of features and of positions inside
-// a product is free, so each thread's mma.sync fragment is made of whole
-// 16-byte pieces of a row: a thread copies exactly the bytes that it will use,
+// So the work is laid out for loads in flight, not for the matrix rate (128 KB
+// under way per SM reach 6.4 TB/s of rows of 128 bytes, 64 KB 4.4 TB/s): every
+// warp runs alone over blocks of 32 positions of one cache head, with a ring of
+// its own that cp.async fills, K and V of a piece in slots of their own so that
+// all but the one in use are under way.  The order of features and of positions
+// inside a product is free, so each thread's mma.sync fragment is made of whole
+// 16-byte parts of a row: a thread copies exactly the bytes that it will use,
 // to places of its own, and reads them back without a conflict or a barrier.
-// No warp waits for another before the end of its share.
+// The warps of a block take heads of the same positions (neighbours in memory)
+// when there is enough work for that, blocks of positions of one head otherwise;
+// only then is there something to add up between them, at the end of an item.
 //
 // Precision: products must be as good as fp32 for fp32 activations.  Operands
 // are split x = hi + lo and, with at most 8 rows, the hi and lo parts of one
@@ -40,7 +44,6 @@ namespace rt {
 namespace {
 
 constexpr int FT = 128, FW = FT / 32;   // threads, warps
-constexpr int FKT = 32 * FW;            // positions per unit: a block of 32 for each warp
 constexpr int M_F16 = 0, M_BF16 = 1, M_TF32 = 2;
 constexpr float RAISE = 8.0f;           // the reference moves when a score passes it by this (log2)
 constexpr float W_SCALE = 64.0f;        // fp16 weights reach 2^8 * 2^6, far from both ends of the type
@@ -62,7 +65,7 @@ struct Few {
     static constexpr int NP = PACK ? 1 : (MODE == M_F16 && !F32ACT ? 1 : 2);
     static constexpr int KSTEP = MODE == M_TF32 ? 8 : 16;              // features per instruction
     static constexpr int KS = DP / KSTEP;
-    static constexpr int SB = 32 / ES < 8 ? 8 : 32 / ES;               // positions per piece: 32, 16, 8
+    static constexpr int SB = 32 / ES;                                 // positions per piece: 32, 16, 8
     static constexpr int SUBS = 32 / SB;
     static constexpr int NT = SB / 8;                                  // score tiles of 8 positions
     static constexpr int KC = DP * ES / 64;                            // 16-byte parts of a K row per thread
@@ -72,14 +75,18 @@ struct Few {
     static constexpr int VE = VB / ES;                                 // features per part
     static constexpr int NO = DP / 8;                                  // output tiles of 8 features
     static constexpr int SLOT = R * DP + 2 * R;                        // floats of an unfinished result
-    static constexpr int Q_BYTES = RT * NQ * KS * 32 * 16;
-    static constexpr int K_BYTES = NT * KC * 512, V_BYTES = VK * VC * 32 * VB;
-    static constexpr int STAGE = K_BYTES + V_BYTES + (Q8 ? 256 : 0) + 16;   // K, V, scales, existing positions
-    static constexpr int STAGES = 2;
+    static constexpr bool Q_REGS = MODE != M_TF32 && RT * NQ == 1;     // query fragments in registers (32 of them)
+    // otherwise in shared memory, a thread's own: tf32 as the values themselves
+    // (hi and lo are made again for each use), 16 bits as the fragments
+    static constexpr int Q_BYTES = Q_REGS ? 0 : MODE == M_TF32 ? KS * (PACK ? 1 : 2) * 32 * 8 : RT * NQ * KS * 32 * 16;
+    static constexpr int HALF = NT * KC * 512;                         // K, or V, of a piece
+    static_assert(HALF == VK * VC * 32 * VB, "K and V alike");
+    static constexpr int SLOT_BYTES = HALF + (Q8 ? 128 : 0) + 16;       // and scales, and which positions exist
+    static constexpr int SLOTS = 16 * 1024 / HALF < 8 ? 16 * 1024 / HALF : 8;
     static constexpr int RS = DP == 128 ? 152 : 72;                    // words of a row in the join: 9 per output tile, 8 (mod 16) in all
-    static constexpr int JOIN = FW * R * (RS + 2) * 4;                 // sums of the warps, over the stages
-    static constexpr int BODY = FW * STAGES * STAGE > JOIN ? FW * STAGES * STAGE : JOIN;
-    static constexpr int SMEM = Q_BYTES + BODY + R * 4 + 64;
+    static constexpr int JOIN = FW * R * (RS + 2) * 4;                 // sums of the warps, over the rings
+    static constexpr int BODY = FW * SLOTS * SLOT_BYTES > JOIN ? FW * SLOTS * SLOT_BYTES : JOIN;
+    static constexpr int SMEM = FW * Q_BYTES + BODY + 64;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -158,53 +165,45 @@ __device__ __forceinline__ void read_part(uint32_t (&r)[2], uint32_t at) {
     asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
 }
 
-// Where feature f of a query fragment goes: step and thread-in-quad, matching
-// the parts K is copied in (features of a thread per step: 4 for the 16-bit
-// products, 2 for tf32).
-template <class F>
-struct QMap {
-    static constexpr int PER = F::MODE == M_TF32 ? 2 : 4;
-    static constexpr int STEPS = 16 / F::ES / PER;          // steps per 16-byte part
-    static __device__ __forceinline__ int step(int f) { return f / (64 / F::ES) * STEPS + f % (16 / F::ES) / PER; }
-    static __device__ __forceinline__ int quad(int f) { return f % (64 / F::ES) / (16 / F::ES); }
-};
-
 template <int CT, bool F32ACT, int DP, int R>
 __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __grid_constant__ PagedArgs p) {
     using F = Few<CT, F32ACT, DP, R>;
     constexpr int MODE = F::MODE, NR = F::NR, RT = F::RT;
     extern __shared__ __align__(16) uint8_t smem[];
-    uint4* qs = reinterpret_cast<uint4*>(smem);                             // [RT][NQ][KS][32]
-    float* os = reinterpret_cast<float*>(smem + F::Q_BYTES);                // [FW][R][RS], over the stages
+    float* os = reinterpret_cast<float*>(smem + FW * F::Q_BYTES);           // [FW][R][RS], over the rings
     float* ml = os + FW * R * F::RS;                                        // [FW][2][R]
-    float* qscale = reinterpret_cast<float*>(smem + F::Q_BYTES + F::BODY);  // [R]
-    int* sched = reinterpret_cast<int*>(qscale + R);
+    int* sched = reinterpret_cast<int*>(smem + FW * F::Q_BYTES + F::BODY);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* const stages = smem + F::Q_BYTES + warp * F::STAGES * F::STAGE;
-    const uint32_t stages_at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
+    uint8_t* const my_q = smem + warp * F::Q_BYTES;
+    uint8_t* const ring = smem + FW * F::Q_BYTES + warp * F::SLOTS * F::SLOT_BYTES;
+    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
     const RtKvCache& c = p.a.cache;
     const int D = c.head_dim;
     const bool act_bf16 = p.a.dtype == RT_BF16;
+    const int key_warps = FW / p.head_group, w_head = warp & (p.head_group - 1), w_key = warp / p.head_group;
+    const int stride = 32 * key_warps;                                      // positions of a key tile
 
     asm volatile("griddepcontrol.launch_dependents;");
     PagedCursor cur;
     int u, per, total;
-    if (!paged_schedule<FT, R, FKT>(p, blockIdx.x, gridDim.x, sched, cur, u, per, total)) return;
+    const bool some = paged_schedule<FT, R>(p, blockIdx.x, gridDim.x, sched, cur, u, per, total);
+    paged_note<R>(p, some, cur, u, per);
+    if (!some) return;
     const int u_end = (int)min((int64_t)u + per, (int64_t)total);
 
     while (u < u_end) {
         const int seg = p.whole ? cur.t.count : min(cur.t.count - cur.i, u_end - u);
         const PagedSeq& s = cur.s;
-        const int row0 = cur.qt * R, rows = min(R, s.n * p.group - row0);
-        const int k_begin = (cur.t.t0 + cur.i) * FKT, k_end = min((cur.t.t0 + cur.i + seg) * FKT, cur.t.hi);
-        const uint8_t* kb = static_cast<const uint8_t*>(c.k) + cur.h * c.stride[2] * F::ES;
-        const uint8_t* vb = static_cast<const uint8_t*>(c.v) + cur.h * c.stride[2] * F::ES;
+        const int row0 = cur.qt * R, rows = min(R, s.n * p.group - row0), head = cur.h * p.head_group + w_head;
+        const int k_begin = (cur.t.t0 + cur.i) << p.key_shift, k_end = min((cur.t.t0 + cur.i + seg) << p.key_shift, cur.t.hi);
+        const uint8_t* kb = static_cast<const uint8_t*>(c.k) + head * c.stride[2] * F::ES;
+        const uint8_t* vb = static_cast<const uint8_t*>(c.v) + head * c.stride[2] * F::ES;
         const int* table = p.a.page_table + s.b * p.a.table_stride;
-        const int first = k_begin + warp * 32;                               // of this warp's blocks
-        const int pieces = first < k_end ? (k_end - first + FKT - 1) / FKT * F::SUBS : 0;
+        const int first = k_begin + w_key * 32;                              // of this warp's blocks
+        const int pieces = first < k_end ? (k_end - first + stride - 1) / stride * F::SUBS : 0;
 
-        // ---- copies: a lane looks up one position of a block, a block ahead ----
-        int copied = 0, page_next = -1;
+        // ---- copies: K and V of piece after piece; a lane looks up one position of a block, a block ahead ----
+        int copied = 0, slot_c = 0, page_next = -1, sp = 0;                  // sp: this lane's scale
         uint32_t off = ~0u;                                                  // this lane's row, units of 16 bytes
         auto page_of = [&](int pos) -> int {
             if (pos >= k_end || pos < cur.t.lo) return -1;
@@ -213,53 +212,56 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             const int page = table[ip];
             return page < 0 ? 0x7fffffff : page;
         };
-        auto copy_piece = [&]() {
-            if (copied < pieces) {
-                const int sub = copied % F::SUBS, pos = first + copied / F::SUBS * FKT + lane;
-                const uint32_t at = stages_at + copied % F::STAGES * F::STAGE;
-                if (sub == 0) {
+        auto copy_half = [&]() {
+            if (copied < 2 * pieces) {
+                const int sub = (copied >> 1) % F::SUBS, pos = first + (copied >> 1) / F::SUBS * stride + lane;
+                const bool is_v = copied & 1;
+                const uint32_t at = ring_at + slot_c * F::SLOT_BYTES;
+                if (sub == 0 && !is_v) {
                     off = ~0u;
-                    int64_t sp = 0;
                     if (page_next >= c.n_pages) {
                         atomicCAS(p.err, 0, KERR_PAGE);
                     } else if (page_next >= 0) {
                         int ip, slot;
                         paged_split(p, pos, ip, slot);
                         off = (uint32_t)((page_next * c.stride[0] + slot * c.stride[1]) * F::ES >> 4);
-                        if constexpr (F::Q8) sp = page_next * c.scale_stride[0] + slot * c.scale_stride[1] + cur.h * c.scale_stride[2];
+                        if constexpr (F::Q8) sp = (int)(page_next * c.scale_stride[0] + slot * c.scale_stride[1] + head * c.scale_stride[2]);
                     }
-                    page_next = page_of(pos + FKT);
-                    if constexpr (F::Q8) {
-                        copy_part<4>(at + F::K_BYTES + F::V_BYTES + lane * 4, reinterpret_cast<const uint8_t*>(c.k_scale + sp), off != ~0u);
-                        copy_part<4>(at + F::K_BYTES + F::V_BYTES + 128 + lane * 4, reinterpret_cast<const uint8_t*>(c.v_scale + sp), off != ~0u);
-                    }
+                    page_next = page_of(pos + stride);
                 }
-                const uint32_t there = __ballot_sync(0xffffffffu, off != ~0u);
-                if (lane == 0) *reinterpret_cast<uint32_t*>(stages + copied % F::STAGES * F::STAGE + F::STAGE - 16) = there;
+                if constexpr (F::Q8)
+                    copy_part<4>(at + F::HALF + lane * 4, reinterpret_cast<const uint8_t*>((is_v ? c.v_scale : c.k_scale) + sp), off != ~0u);
+                if (!is_v) {
+                    const uint32_t there = __ballot_sync(0xffffffffu, off != ~0u) >> (sub * F::SB);
+                    if (lane == 0) *reinterpret_cast<uint32_t*>(ring + slot_c * F::SLOT_BYTES + F::SLOT_BYTES - 16) = there;
+                }
                 // a row's address once, its parts at constant distances; rows that no one sees
                 // give zeros
                 auto rows_of = [&](auto whole) {
+                    if (!is_v) {
 #pragma unroll
-                    for (int n = 0; n < F::NT; n++) {
-                        const uint32_t o = __shfl_sync(0xffffffffu, off, sub * F::SB + n * 8 + g);
-                        const bool live = o != ~0u;
-                        const uint8_t* row = kb + (live ? ((uint64_t)o << 4) + t * 16 : 0);
+                        for (int n = 0; n < F::NT; n++) {
+                            const uint32_t o = __shfl_sync(0xffffffffu, off, sub * F::SB + n * 8 + g);
+                            const bool live = o != ~0u;
+                            const uint8_t* row = kb + (live ? ((uint64_t)o << 4) + t * 16 : 0);
 #pragma unroll
-                        for (int i = 0; i < F::KC; i++) {
-                            const bool in = decltype(whole)::value || i * 64 + t * 16 < D * F::ES;
-                            copy_part<16>(at + ((n * F::KC + i) * 32 + lane) * 16, in ? row + i * 64 : kb, live && in);
+                            for (int i = 0; i < F::KC; i++) {
+                                const bool in = decltype(whole)::value || i * 64 + t * 16 < D * F::ES;
+                                copy_part<16>(at + ((n * F::KC + i) * 32 + lane) * 16, in ? row + i * 64 : kb, live && in);
+                            }
                         }
-                    }
+                    } else {
 #pragma unroll
-                    for (int n = 0; n < F::VK; n++) {   // 16-bit products: rows 2t, 2t+1, 2t+8, 2t+9 of each 16; tf32: 2t, 2t+1 of each 8
-                        const int key = MODE == M_TF32 ? (n >> 1) * 8 + 2 * t + (n & 1) : (n >> 2) * 16 + ((n >> 1) & 1) * 8 + 2 * t + (n & 1);
-                        const uint32_t o = __shfl_sync(0xffffffffu, off, sub * F::SB + key);
-                        const bool live = o != ~0u;
-                        const uint8_t* row = vb + (live ? ((uint64_t)o << 4) + g * F::VB : 0);
+                        for (int n = 0; n < F::VK; n++) {   // 16-bit products: rows 2t, 2t+1, 2t+8, 2t+9 of each 16; tf32: 2t, 2t+1 of each 8
+                            const int key = MODE == M_TF32 ? (n >> 1) * 8 + 2 * t + (n & 1) : (n >> 2) * 16 + ((n >> 1) & 1) * 8 + 2 * t + (n & 1);
+                            const uint32_t o = __shfl_sync(0xffffffffu, off, sub * F::SB + key);
+                            const bool live = o != ~0u;
+                            const uint8_t* row = vb + (live ? ((uint64_t)o << 4) + g * F::VB : 0);
 #pragma unroll
-                        for (int i = 0; i < F::VC; i++) {
-                            const bool in = decltype(whole)::value || i * 8 * F::VB + g * F::VB < D * F::ES;
-                            copy_part<F::VB>(at + F::K_BYTES + ((n * F::VC + i) * 32 + lane) * F::VB, in ? row + i * 8 * F::VB : vb, live && in);
+                            for (int i = 0; i < F::VC; i++) {
+                                const bool in = decltype(whole)::value || i * 8 * F::VB + g * F::VB < D * F::ES;
+                                copy_part<F::VB>(at + ((n * F::VC + i) * 32 + lane) * F::VB, in ? row + i * 8 * F::VB : vb, live && in);
+                            }
                         }
                     }
                 };
@@ -268,107 +270,116 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             copied++;
+            slot_c = slot_c + 1 == F::SLOTS ? 0 : slot_c + 1;
         };
         page_next = page_of(first + lane);
-#pragma unroll
-        for (int i = 0; i < F::STAGES - 1; i++) copy_piece();
+#pragma unroll 1
+        for (int i = 0; i < F::SLOTS - 1; i++) copy_half();
 
-        // ---- query fragments (the first pieces are on their way): 8 features a thread ----
+        // ---- query fragments (the first pieces are on their way): a thread reads the features that it uses ----
         const float base = p.a.scale * 1.4426950408889634f;
-        constexpr int LQ = DP / 8;                          // threads of a row
+        float up[NR];
+        uint4 qr[F::Q_REGS ? F::KS : 1];
+        {
+            constexpr int PF = 16 / F::ES, CH = DP / (4 * PF);   // consecutive features of a thread, and how often
+            float x[NR][CH * PF];
 #pragma unroll
-        for (int r0 = 0; r0 < R; r0 += FT / LQ) {
-            const int r = r0 + tid / LQ, d = tid % LQ * 8;
-            if (R < FT / LQ && r >= R) break;               // (whole rows, which lie in whole half warps)
-            float x[8];
+            for (int k = 0; k < NR; k++) {
+                const int r = g + 8 * k, rr = row0 + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
+                const int64_t at = (int64_t)(s.first + tok) * p.a.q_stride[0] + hq * p.a.q_stride[1];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.0f;
-            if (r < rows && d < D) {
-                const int rr = row0 + r, tok = rr / p.group, hq = cur.h * p.group + rr - tok * p.group;
-                const int64_t at = (int64_t)(s.first + tok) * p.a.q_stride[0] + hq * p.a.q_stride[1] + d;
-                if (act_bf16) {
-                    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.a.q) + at;
-                    if (p.vec_q) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(q);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                for (int i = 0; i < CH * PF; i += 4) {
+                    const int d = i / PF * 4 * PF + t * PF + i % PF;
+                    float* v = x[k] + i;
+                    v[0] = v[1] = v[2] = v[3] = 0.0f;
+                    if (r < rows && d < D) {
+                        if (act_bf16) {
+                            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.a.q) + at + d;
+                            if (p.vec_q) {
+                                const uint2 w = *reinterpret_cast<const uint2*>(q);
+                                v[0] = __uint_as_float(w.x << 16);
+                                v[1] = __uint_as_float(w.x & 0xffff0000u);
+                                v[2] = __uint_as_float(w.y << 16);
+                                v[3] = __uint_as_float(w.y & 0xffff0000u);
+                            } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            x[2 * i] = __uint_as_float(w[i] << 16);
-                            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                                for (int j = 0; j < 4; j++) v[j] = __bfloat162float(q[j]);
+                            }
+                        } else {
+                            const float* q = static_cast<const float*>(p.a.q) + at + d;
+                            if (p.vec_q) {
+                                const float4 w = *reinterpret_cast<const float4*>(q);
+                                v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) v[j] = q[j];
+                            }
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = __bfloat162float(q[i]);
-                    }
-                } else {
-                    const float* q = static_cast<const float*>(p.a.q) + at;
-                    if (p.vec_q) {
-                        const float4 v = *reinterpret_cast<const float4*>(q), w = *reinterpret_cast<const float4*>(q + 4);
-                        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-                        x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = q[i];
                     }
                 }
             }
-            if constexpr (MODE == M_F16) {
-                float m = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
-                const uint32_t mates = (LQ == 16 ? 0xffffu : 0xffu) << (lane / LQ * LQ);
-                m = __uint_as_float(__reduce_max_sync(mates, __float_as_uint(m)));
-                const float up = pow2i(f16_scale_exp(m));
-                if (tid % LQ == 0) qscale[r] = up;
+            for (int k = 0; k < NR; k++) {
+                up[k] = 1.0f;
+                if constexpr (MODE == M_F16) {
+                    float m = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] *= up;
+                    for (int i = 0; i < CH * PF; i++) m = fmaxf(m, fabsf(x[k][i]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    up[k] = pow2i(f16_scale_exp(m));
+#pragma unroll
+                    for (int i = 0; i < CH * PF; i++) x[k][i] *= up[k];
+                }
             }
-            using M = QMap<F>;
-            uint32_t* q = reinterpret_cast<uint32_t*>(qs + r / 16 * F::NQ * F::KS * 32);
+            if constexpr (MODE == M_TF32) {
 #pragma unroll
-            for (int i = 0; i < 8; i += M::PER) {
-                uint32_t hi[2], lo[2];
-                if constexpr (MODE == M_TF32) {
+                for (int st = 0; st < F::KS; st++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        hi[j] = tf32_hi(__float_as_uint(x[i + j]));
-                        lo[j] = tf32_lo(__float_as_uint(x[i + j]));
+                    for (int k = 0; k < NR; k++)
+                        *reinterpret_cast<float2*>(my_q + ((st * NR + k) * 32 + lane) * 8) = make_float2(x[k][2 * st], x[k][2 * st + 1]);
+            } else {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int st = 0; st < F::KS; st++) {
+                        uint32_t hi[2][2], lo[2][2];   // [row half][register]
+#pragma unroll
+                        for (int h = 0; h < (F::PACK ? 1 : 2); h++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++) split_pair<MODE>(x[2 * rt + h][4 * st + 2 * j], x[2 * rt + h][4 * st + 2 * j + 1], hi[h][j], lo[h][j]);
+                        const uint4 first_part = F::PACK ? make_uint4(hi[0][0], lo[0][0], hi[0][1], lo[0][1])
+                                                         : make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
+                        if constexpr (F::Q_REGS) {
+                            qr[st] = first_part;
+                        } else {
+                            uint4* q = reinterpret_cast<uint4*>(my_q) + (rt * F::NQ * F::KS + st) * 32 + lane;
+                            *q = first_part;
+                            if constexpr (F::NQ == 2) q[F::KS * 32] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
+                        }
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 2; j++) split_pair<MODE>(x[i + 2 * j], x[i + 2 * j + 1], hi[j], lo[j]);
-                }
-                uint32_t* e = q + (M::step(d + i) * 32 + r % 8 * 4 + M::quad(d + i)) * 4;
-                if constexpr (F::PACK) {
-                    *reinterpret_cast<uint4*>(e) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
-                } else {
-                    const int half = r >> 3 & 1;
-                    e[half] = hi[0];
-                    e[half + 2] = hi[1];
-                    if constexpr (F::NQ == 2) {
-                        e[F::KS * 128 + half] = lo[0];
-                        e[F::KS * 128 + half + 2] = lo[1];
-                    }
-                }
             }
         }
-        __syncthreads();
 
         // ---- this thread's rows: g (+ 8, + 16, ...) ----
         float c_row[NR], m_ref[NR], l[NR];
         int lo_row[NR], hi_row[NR];
-        bool mixed = false;
+        int all_lo = 0, all_hi = 0x7fffffff;   // positions that every row of the tile sees
 #pragma unroll
         for (int i = 0; i < NR; i++) {
             const int r = g + 8 * i, tok = (row0 + r) / p.group, at = s.L - s.n + tok;
-            c_row[i] = MODE == M_F16 ? base / qscale[r] : base;
+            c_row[i] = base / up[i];
             m_ref[i] = -INFINITY;
             l[i] = 0.0f;
             lo_row[i] = p.a.window > 0 ? max(0, at - p.a.window + 1) : 0;
-            hi_row[i] = r < rows ? (p.a.causal ? min(s.L, at + 1) : s.L) : 0;
-            mixed |= r < rows && (lo_row[i] > cur.t.lo || hi_row[i] < cur.t.hi);
+            hi_row[i] = p.a.causal ? max(0, min(s.L, at + 1)) : s.L;
+            if (r < rows) {
+                all_lo = max(all_lo, lo_row[i]);
+                all_hi = min(all_hi, hi_row[i]);
+            }
         }
-        mixed = __any_sync(0xffffffffu, mixed);   // rows that see different positions share this tile
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
         float o[RT][F::NO][4];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
@@ -377,36 +388,21 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
 #pragma unroll
                 for (int j = 0; j < 4; j++) o[rt][i][j] = 0.0f;
         float vs_max = 0.0f;   // 8-bit: the value scale that weights are expressed in
+        int slot = 0;
 
 #pragma unroll 1
         for (int piece = 0; piece < pieces; piece++) {
-            copies_wait<F::STAGES - 2>();
-            __syncwarp();                       // scales and notes of other lanes; all are done with the stage that is refilled
-            copy_piece();
-            const uint8_t* stage = stages + piece % F::STAGES * F::STAGE;
-            const uint32_t at = stages_at + piece % F::STAGES * F::STAGE;
-            const int sub = piece % F::SUBS, pos = first + piece / F::SUBS * FKT + sub * F::SB;
-            const uint32_t ok = *reinterpret_cast<const uint32_t*>(stage + F::STAGE - 16) >> (sub * F::SB);
-            constexpr uint32_t ALL = F::SB == 32 ? 0xffffffffu : (1u << F::SB) - 1;
+            copies_wait<F::SLOTS - 2>();
+            __syncwarp();                       // scales and notes of other lanes; all are done with the slot that is refilled
+            copy_half();
+            const int sub = piece % F::SUBS, pos = first + piece / F::SUBS * stride + sub * F::SB;
+            const uint32_t k_at = ring_at + slot * F::SLOT_BYTES;
+            const float* k_scale = reinterpret_cast<const float*>(ring + slot * F::SLOT_BYTES + F::HALF);
+            const uint32_t ok = *reinterpret_cast<const uint32_t*>(ring + slot * F::SLOT_BYTES + F::SLOT_BYTES - 16);
+            slot = slot + 1 == F::SLOTS ? 0 : slot + 1;
+            constexpr uint32_t ALL = F::SB == 32 ? 0xffffffffu : (1u << (F::SB & 31)) - 1;
+            const bool mixed = pos < all_lo || pos + F::SB > all_hi;           // rows see different positions of the piece
             const bool masked = mixed || (ok & ALL) != ALL;
-            const float* k_scale = reinterpret_cast<const float*>(stage + F::K_BYTES + F::V_BYTES);
-            const float* v_scale = k_scale + 32;
-            float to_w = 0.0f;
-            if constexpr (F::Q8) {
-                const float mine = v_scale[lane];
-                const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, mine > 0.0f && mine < INFINITY ? __float_as_uint(mine) : 0u));
-                if (top > vs_max) {   // with room for four times more, so that it seldom moves
-                    const float to = 4.0f * top, f = vs_max / to;
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                        for (int i = 0; i < F::NO; i++)
-#pragma unroll
-                            for (int j = 0; j < 4; j++) o[rt][i][j] *= f;
-                    vs_max = to;
-                }
-                to_w = vs_max > 0.0f ? W_SCALE / vs_max : 0.0f;
-            }
             // ---- scores ----
             float sc[RT][F::NT][4];
 #pragma unroll
@@ -420,17 +416,33 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             for (int i = 0; i < F::KC; i++) {
                 uint32_t kr[F::NT][4];
 #pragma unroll
-                for (int n = 0; n < F::NT; n++) read_part(kr[n], at + ((n * F::KC + i) * 32 + lane) * 16);
+                for (int n = 0; n < F::NT; n++) read_part(kr[n], k_at + ((n * F::KC + i) * 32 + lane) * 16);
 #pragma unroll
                 for (int e = 0; e < PER; e++) {
+                    const int st = i * PER + e;
                     uint32_t a[RT][F::NQ][4];
+                    if constexpr (MODE == M_TF32) {
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++)
+                        for (int k = 0; k < NR; k++) {
+                            const float2 x = *reinterpret_cast<const float2*>(my_q + ((st * NR + k) * 32 + lane) * 8);
+                            const uint32_t v[2] = {__float_as_uint(x.x), __float_as_uint(x.y)};
 #pragma unroll
-                        for (int k = 0; k < F::NQ; k++) {
-                            const uint4 x = qs[((rt * F::NQ + k) * F::KS + i * PER + e) * 32 + lane];
-                            a[rt][k][0] = x.x; a[rt][k][1] = x.y; a[rt][k][2] = x.z; a[rt][k][3] = x.w;
+                            for (int j = 0; j < 2; j++) {
+                                a[0][0][2 * j + (F::PACK ? 0 : k)] = tf32_hi(v[j]);
+                                if constexpr (F::PACK) a[0][0][2 * j + 1] = tf32_lo(v[j]);
+                                else a[0][F::NQ - 1][2 * j + k] = tf32_lo(v[j]);
+                            }
                         }
+                    } else {
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                            for (int k = 0; k < F::NQ; k++) {
+                                const uint4 x = F::Q_REGS ? qr[F::Q_REGS ? st : 0]
+                                                          : reinterpret_cast<const uint4*>(my_q)[((rt * F::NQ + k) * F::KS + st) * 32 + lane];
+                                a[rt][k][0] = x.x; a[rt][k][1] = x.y; a[rt][k][2] = x.z; a[rt][k][3] = x.w;
+                            }
+                    }
 #pragma unroll
                     for (int n = 0; n < F::NT; n++) {
                         uint32_t b0, b1;
@@ -478,6 +490,29 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
                         mx[i] = fmaxf(mx[i], x);
                     }
                 }
+            }
+            // V of the piece; K's slot is free once its scales are used
+            copies_wait<F::SLOTS - 2>();
+            __syncwarp();
+            copy_half();
+            const uint32_t v_at = ring_at + slot * F::SLOT_BYTES;
+            const float* v_scale = reinterpret_cast<const float*>(ring + slot * F::SLOT_BYTES + F::HALF);
+            slot = slot + 1 == F::SLOTS ? 0 : slot + 1;
+            float to_w = 0.0f;
+            if constexpr (F::Q8) {
+                const float mine = v_scale[lane];
+                const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, mine > 0.0f && mine < INFINITY ? __float_as_uint(mine) : 0u));
+                if (top > vs_max) {   // with room for four times more, so that it seldom moves
+                    const float to = 4.0f * top, f = vs_max / to;
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                        for (int i = 0; i < F::NO; i++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[rt][i][j] *= f;
+                    vs_max = to;
+                }
+                to_w = vs_max > 0.0f ? W_SCALE / vs_max : 0.0f;
             }
             bool raise = false;
 #pragma unroll
@@ -534,7 +569,7 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
 #pragma unroll 1
                     for (int i = 0; i < F::VK * F::VC; i++) {
                         uint32_t x[4];
-                        read_part(x, at + F::K_BYTES + (i * 32 + lane) * 16);
+                        read_part(x, v_at + (i * 32 + lane) * 16);
 #pragma unroll
                         for (int r = 0; r < 4; r++)
                             strange |= (x[r] & 0x7f800000u) == 0x7f800000u || (CT == RT_BF16 && (x[r] & 0x7f80u) == 0x7f80u);
@@ -583,7 +618,7 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
                 for (int i = 0; i < F::VC; i++) {
                     uint32_t vr[VR][F::VB / 4];
 #pragma unroll
-                    for (int n = 0; n < VR; n++) read_part(vr[n], at + F::K_BYTES + (((st * VR + n) * F::VC + i) * 32 + lane) * F::VB);
+                    for (int n = 0; n < VR; n++) read_part(vr[n], v_at + (((st * VR + n) * F::VC + i) * 32 + lane) * F::VB);
                     if constexpr (MODE == M_F16) {
 #pragma unroll
                         for (int r = 0; r < F::VB / 4; r++) {
@@ -670,73 +705,134 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             }
         }
 
-        // ---- join the warps ----
         copies_wait<0>();
-        __syncthreads();                        // nobody needs the stages any more
         const float fo = F::Q8 ? vs_max / W_SCALE : 1.0f;
+        const bool done = cur.i == 0 && seg == cur.t.count;
+        float* parts = p.part + (int64_t)(2 * blockIdx.x + (cur.i == 0)) * p.head_group * F::SLOT;   // (heads of the group)
 #pragma unroll
         for (int i = 0; i < NR; i++) {
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-            if (t == 0) {
-                ml[warp * 2 * R + g + 8 * i] = m_ref[i];
-                ml[warp * 2 * R + R + g + 8 * i] = l[i];
-            }
         }
+        if (key_warps == 1) {
+            // ---- a warp has its head to itself: VE consecutive features of a row at a time ----
 #pragma unroll
-        for (int i = 0; i < F::VC; i++)
+            for (int k = 0; k < NR; k++) {
+                const int r = g + 8 * k;
+                if (r >= rows) continue;
+                const float f = done ? (l[k] == 0.0f ? 0.0f : fo / l[k]) : fo;
+                float* part = parts + w_head * F::SLOT + r * DP;
 #pragma unroll
-            for (int e = 0; e < F::VE; e++)
+                for (int i = 0; i < F::VC; i++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    // word n * 9 + column of the row: a warp's stores and loads meet few conflicts
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int e = 0; e < F::VE; e += 4) {
+                            const int d = i * 8 * F::VE + (2 * t + j) * F::VE + e;
+                            float x[4];
+#pragma unroll
+                            for (int v = 0; v < 4; v++) {
+                                const float* y = o[k / 2][i * F::VE + e + v];
+                                x[v] = (F::PACK ? y[j] + y[2 + j] : y[2 * (k & 1) + j]) * f;
+                            }
+                            if (!done) *reinterpret_cast<float4*>(part + d) = make_float4(x[0], x[1], x[2], x[3]);
+                            else if (d < D) paged_store4(p, s, head, row0 + r, d, x[0], x[1], x[2], x[3]);
+                        }
+                if (t == 0) {
+                    if (!done) parts[w_head * F::SLOT + R * DP + r] = m_ref[k], parts[w_head * F::SLOT + R * DP + R + r] = l[k];
+                    else paged_store_lse(p, s, head, row0 + r, m_ref[k], l[k]);
+                }
+            }
+        } else {
+            // ---- add up the warps of a head ----
+            __syncthreads();                    // nobody needs the rings any more
+            if (t == 0) {
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    ml[warp * 2 * R + g + 8 * i] = m_ref[i];
+                    ml[warp * 2 * R + R + g + 8 * i] = l[i];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < F::NO; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)   // word n * 9 + column of the row: a warp's stores and loads meet few conflicts
 #pragma unroll
                     for (int k = 0; k < NR; k++) {
-                        const float* x = o[k / 2][i * F::VE + e];
-                        os[(warp * R + g + 8 * k) * F::RS + (i * F::VE + e) * 9 + 2 * t + j] = (F::PACK ? x[j] + x[2 + j] : x[2 * (k & 1) + j]) * fo;
+                        const float* x = o[k / 2][n];
+                        os[(warp * R + g + 8 * k) * F::RS + n * 9 + 2 * t + j] = (F::PACK ? x[j] + x[2 + j] : x[2 * (k & 1) + j]) * fo;
+                    }
+            __syncthreads();
+            for (int e = tid; e < p.head_group * rows * (DP / 4); e += FT) {   // 4 features of a row a thread
+                const int h = e / (rows * (DP / 4)), r = e / (DP / 4) - h * rows, d = e % (DP / 4) * 4;
+                float m = -INFINITY, ls = 0.0f, sum[4] = {0, 0, 0, 0};
+                for (int k = h; k < FW; k += p.head_group) m = fmaxf(m, ml[k * 2 * R + r]);
+                for (int k = h; k < FW; k += p.head_group) {
+                    const float mk = ml[k * 2 * R + r];
+                    if (mk == -INFINITY) continue;                             // (a warp without positions)
+                    const float f = exp2_fast(mk - m);
+                    if (f == 0.0f) continue;
+                    ls += ml[k * 2 * R + R + r] * f;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int n = (d + j) / (8 * F::VE) * F::VE + (d + j) % F::VE, col = (d + j) / F::VE % 8;
+                        sum[j] += os[(k * R + r) * F::RS + n * 9 + col] * f;
                     }
                 }
-        __syncthreads();
-        const bool done = cur.i == 0 && seg == cur.t.count;
-        float* part = p.part + (int64_t)(2 * blockIdx.x + (cur.i == 0)) * F::SLOT;
-        for (int e = tid; e < rows * (DP / 4); e += FT) {   // 4 features of a row a thread
-            const int r = e / (DP / 4), d = e % (DP / 4) * 4;
-            float f[FW], m = -INFINITY, ls = 0.0f, sum[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < FW; k++) {
-                f[k] = ml[k * 2 * R + r];
-                m = fmaxf(m, f[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < FW; k++) {
-                f[k] = f[k] == -INFINITY ? 0.0f : exp2_fast(f[k] - m);   // (a warp without positions)
-                if (f[k] == 0.0f) continue;
-                ls += ml[k * 2 * R + R + r] * f[k];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int n = (d + j) / (8 * F::VE) * F::VE + (d + j) % F::VE, col = (d + j) / F::VE % 8;
-                    sum[j] += os[(k * R + r) * F::RS + n * 9 + col] * f[k];
+                float* part = parts + h * F::SLOT;
+                if (!done) {
+                    *reinterpret_cast<float4*>(part + r * DP + d) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                    if (d == 0) part[R * DP + r] = m, part[R * DP + R + r] = ls;
+                } else if (d < D) {
+                    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+                    paged_store4(p, s, cur.h * p.head_group + h, row0 + r, d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+                    if (d == 0) paged_store_lse(p, s, cur.h * p.head_group + h, row0 + r, m, ls);
                 }
             }
-            if (!done) {
-                *reinterpret_cast<float4*>(part + r * DP + d) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-                if (d == 0) part[R * DP + r] = m, part[R * DP + R + r] = ls;
-            } else if (d < D) {
-                const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-                paged_store4(p, s, cur.h, row0 + r, d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
-                if (d == 0) paged_store_lse(p, s, cur.h, row0 + r, m, ls);
-            }
+            __syncthreads();
         }
-        __syncthreads();
         u += p.whole ? 1 : seg;
-        cur.next_item<R, FKT>(p);
+        cur.next_item<R>(p);
     }
 }
 
-// Calls whose longest sequence fits this many positions run as one launch,
-// every item in one block: the join would cost more than it spreads.
+constexpr int MAX_BLOCKS_PER_SM = 3;
+// How a call is spread.  Calls whose longest sequence fits WHOLE_KEYS positions
+// run as one launch, every item in one block: the join would cost more than it
+// spreads.  Blocks take a group of heads when there are enough items even then
+// (heads of the same positions lie next to each other, and warps have nothing
+// to add up), one head when items have to be cut into many parts.
 constexpr int WHOLE_KEYS = 512;
-constexpr int MIN_UNITS = 2;
+constexpr int MIN_POSITIONS = 256;   // of a block's share
+struct Spread {
+    int rows, head_group, key_shift, blocks;
+    bool whole;
+};
+// Rows of a tile: 8 when that covers a call's rows (a thread then has the
+// weights of one row to make, not of two), 16, or two tiles of 16 over the
+// same keys for one-part products.
+int few_rows(const RtPagedAttention& p) {
+    const bool bf = p.dtype == RT_BF16;
+    const int64_t rows = (int64_t)std::min(p.max_new, p.total_new) * (p.n_q_heads / p.cache.n_heads);
+    if (bf && rows > 16 && p.cache.dtype != RT_F32) return 32;
+    return rows <= 8 ? 8 : 16;
+}
+Spread few_spread(const RtPagedAttention& p, int per_sm) {
+    Spread s;
+    s.rows = few_rows(p);
+    s.whole = p.max_kv <= WHOLE_KEYS;
+    const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(p.max_new, p.total_new)) * (p.n_q_heads / p.cache.n_heads);
+    const int64_t tiles = (int64_t)p.n_seqs * ((rows + s.rows - 1) / s.rows), positions = std::max(p.max_kv, 1);
+    s.head_group = 1;
+    while (!s.whole && s.head_group < FW && p.cache.n_heads % (2 * s.head_group) == 0 &&
+           tiles * (p.cache.n_heads / (2 * s.head_group)) * 6 >= g_num_sms * MAX_BLOCKS_PER_SM)
+        s.head_group *= 2;
+    s.key_shift = s.head_group == 1 ? 7 : s.head_group == 2 ? 6 : 5;
+    const int64_t items = tiles * (p.cache.n_heads / s.head_group);
+    const int64_t shares = s.whole ? items : (items * positions + MIN_POSITIONS - 1) / MIN_POSITIONS;
+    s.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)g_num_sms * per_sm, shares));
+    return s;
+}
 
 template <int CT, bool F32ACT, int DP, int R>
 int few_blocks_per_sm() {
@@ -748,42 +844,24 @@ int few_blocks_per_sm() {
             cudaGetLastError();
             k = 1;
         }
-        return k;
+        return std::min(k, MAX_BLOCKS_PER_SM);
     }();
     return n;
-}
-constexpr int MAX_BLOCKS_PER_SM = 4;
-
-// Blocks of a call: no more than fit the GPU at once, no more than it has work for.
-int few_blocks(const RtPagedAttention& p, int R, int per_sm, bool whole) {
-    const int64_t group = p.n_q_heads / p.cache.n_heads;
-    const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(p.max_new, p.total_new)) * group;
-    const int64_t items = (int64_t)p.n_seqs * p.cache.n_heads * ((rows + R - 1) / R);
-    const int64_t units = whole ? items : items * ((p.max_kv + FKT - 1) / FKT);
-    return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)g_num_sms * per_sm, whole ? units : (units + MIN_UNITS - 1) / MIN_UNITS));
 }
 
 template <int CT, bool F32ACT, int DP, int R>
 Status few_as(PagedArgs& p, void* ws, cudaStream_t st) {
     using F = Few<CT, F32ACT, DP, R>;
-    const int per_sm = std::min(MAX_BLOCKS_PER_SM, few_blocks_per_sm<CT, F32ACT, DP, R>());
-    const int blocks = few_blocks(p.a, R, per_sm, p.whole);
-    p.part = static_cast<float*>(ws);
-    p.min_units = p.whole ? 1 : MIN_UNITS;
-    paged_few_kernel<CT, F32ACT, DP, R><<<blocks, FT, F::SMEM, st>>>(p);
+    const Spread s = few_spread(p.a, few_blocks_per_sm<CT, F32ACT, DP, R>());
+    paged_set_workspace(p, ws, s.blocks);
+    p.whole = s.whole;
+    p.key_shift = s.key_shift;
+    p.head_group = s.head_group;
+    p.head_groups = p.a.cache.n_heads / s.head_group;
+    p.min_units = s.whole ? 1 : MIN_POSITIONS >> s.key_shift;
+    paged_few_kernel<CT, F32ACT, DP, R><<<s.blocks, FT, F::SMEM, st>>>(p);
     RT_LAUNCH_CHECK();
-    if (p.whole || blocks == 1) return Status::ok();
-    return launch_paged_join<DP, R, FKT>(p, blocks, st);
-}
-
-// Rows of a tile: 8 when that covers a call's rows and the hi / lo parts need
-// the other 8; single-part products take 16 at the same cost, and two tiles of
-// 16 over the same keys when there are more.
-int few_rows(const RtPagedAttention& p) {
-    const bool q8 = p.cache.dtype == RT_I8 || p.cache.dtype == RT_F8E4M3, bf = p.dtype == RT_BF16;
-    const int64_t rows = (int64_t)std::min(p.max_new, p.total_new) * (p.n_q_heads / p.cache.n_heads);
-    if (bf && rows > 16 && p.cache.dtype != RT_F32) return 32;
-    return rows <= 8 && !(q8 && bf) ? 8 : 16;
+    return s.whole || s.blocks == 1 ? Status::ok() : launch_paged_join<DP, R>(p, s.blocks, st);
 }
 
 template <int CT, bool F32ACT, int R>
@@ -792,27 +870,23 @@ Status few_dim(PagedArgs& p, void* ws, cudaStream_t st) {
 }
 template <int CT, bool F32ACT>
 Status few_sizes(PagedArgs& p, void* ws, cudaStream_t st) {
-    constexpr bool Q8 = CT == RT_I8 || CT == RT_F8E4M3;
     const int rows = few_rows(p.a);
     if constexpr (!F32ACT)
         if (rows == 32) return few_dim<CT, F32ACT, 32>(p, ws, st);
-    if constexpr (!Q8 || F32ACT)
-        if (rows == 8) return few_dim<CT, F32ACT, 8>(p, ws, st);
+    if (rows == 8) return few_dim<CT, F32ACT, 8>(p, ws, st);
     return few_dim<CT, F32ACT, 16>(p, ws, st);
 }
-
-bool few_whole(const RtPagedAttention& p) { return p.max_kv <= WHOLE_KEYS; }
 
 }  // namespace
 
 size_t paged_few_workspace(const RtPagedAttention& p) {
-    if (few_whole(p)) return 0;
-    const int R = few_rows(p), DP = p.cache.head_dim > 64 ? 128 : 64;
-    return (size_t)few_blocks(p, R, MAX_BLOCKS_PER_SM, false) * 2 * (R * DP + 2 * R) * sizeof(float);
+    const Spread s = few_spread(p, MAX_BLOCKS_PER_SM);
+    if (s.whole) return 0;
+    const int DP = p.cache.head_dim > 64 ? 128 : 64;
+    return paged_workspace(s.blocks, s.head_group, s.rows * DP + 2 * s.rows);
 }
 
 Status launch_paged_few(PagedArgs& p, void* ws, cudaStream_t st) {
-    p.whole = few_whole(p.a);
     const bool f32 = p.a.dtype == RT_F32;
     switch (p.a.cache.dtype) {
         case RT_F32: return few_sizes<RT_F32, true>(p, ws, st);   // (bf16 activations need the same products)

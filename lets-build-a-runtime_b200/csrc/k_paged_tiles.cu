@@ -99,6 +99,14 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
     const int n = live ? 16 : 0;   // 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Arrives once on `bar` (an arrival that its count includes) when the copies of
+// this thread so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
     const int n = live ? 4 : 0;
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -198,12 +206,14 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
     asm volatile("griddepcontrol.launch_dependents;");
     PagedCursor cur;
     int u, per, total;
-    if (!paged_schedule<TT, T::R, TKT>(p, blockIdx.x, gridDim.x, reinterpret_cast<int*>(smem), cur, u, per, total)) return;
+    const bool some = paged_schedule<TT, T::R>(p, blockIdx.x, gridDim.x, reinterpret_cast<int*>(smem), cur, u, per, total);
+    paged_note<T::R>(p, some, cur, u, per);
+    if (!some) return;
     const int u_end = (int)min((int64_t)u + per, (int64_t)total);
 
     if (tid == 0) {
         for (int i = 0; i < T::SLOTS; i++) {
-            ptx::mbar_init(&bar.full[i], 128);
+            ptx::mbar_init(&bar.full[i], T::DIRECT ? 128 + 4 : 128);   // (+ 4: the warps' notes)
             ptx::mbar_init(&bar.empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -229,27 +239,35 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
 
     if (warp < 4) {
         // ------------------------------------------------ K and V from the pages
-        // A lane looks up one position of the warp's 32, all lanes then copy rows:
-        // cp.async, straight into the ring (bf16 all the way) or, in pieces of RB
-        // loads a lane, into a raw ring from which the same thread converts its own
-        // bytes.  Copies run AHEAD pieces in front of what is handed over.
+        // A lane looks up one position of the warp's 32, all lanes then copy rows with
+        // cp.async: bf16 all the way straight into the ring, where the copies themselves
+        // arrive on the slot's barrier; the rest, in pieces of RB loads a lane, into a raw
+        // ring from which the same thread converts its own bytes, AHEAD pieces later.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_LOAD));
         bool ok = true;
         const uint32_t ring = ptx::smem_u32(smem + T::OFF_RING), raw = ptx::smem_u32(smem + T::OFF_RAW) + tid * 16;
         constexpr int LANES = D * T::ES / 16, ROWS = 32 / LANES;          // lanes of a row, rows of a warp's load
         constexpr int LOADS = 32 / ROWS;                                  // loads of a warp's 32 rows
         constexpr int PIECES = T::DIRECT ? 1 : LOADS / T::RB, PER = LOADS / PIECES;
-        constexpr int AHEAD = T::DIRECT ? T::SLOTS - 2 : T::NRAW - 1;
         const int sub_row = lane / LANES, piece16 = lane % LANES;
-        volatile uint32_t* meta = bar.meta[warp];                         // by load & 7: is_v | mixed << 1 | tile << 2
-        volatile uint32_t* there = bar.there[warp];                       // by load & 7: positions that exist
+        const uint8_t* const k_lane = static_cast<const uint8_t*>(c.k) + piece16 * 16;
+        const uint8_t* const v_lane = static_cast<const uint8_t*>(c.v) + piece16 * 16;
+        // Place of this lane's part of row i * ROWS + sub_row of the warp's 32 in a tile of
+        // 2-byte elements: the swizzle repeats every 8 rows.
+        constexpr int OUT_B = T::VP == 2 ? 8 : T::Q8 ? 32 : 16, TURN = 8 / ROWS ? 8 / ROWS : 1;   // bytes of the part; loads of 8 rows
+        uint32_t place[TURN];
+#pragma unroll
+        for (int i = 0; i < TURN; i++) place[i] = tile_at(warp * 32 + i * ROWS + sub_row, piece16 * OUT_B);
+        auto place_of = [&](int i) { return place[i % TURN] + (uint32_t)(i / TURN) * 1024u; };
 
         // ---- the copies ----
         Segment g = segment_of<T>(p, cur, u, u_end);
-        int idx = 0, tile_base = 0, n_copy = 0, part = 0;   // load of the segment, tiles before it, loads begun, piece
+        int idx = 0, tile_base = 0, n_copy = 0;             // load of the segment, tiles before it, loads begun
         uint32_t off0 = ~0u, off1 = ~0u, off_now = ~0u;     // this lane's row of even / odd tiles, units of 16 bytes
         int sp0 = 0, sp1 = 0, sp_now = 0, page_next = 0;    // its scale; the page of the next key tile
-        bool is_v = false;
+        bool is_v = false, mixed = false;
+        int tile_no = 0;
+        uint32_t live = 0;                                  // positions of the warp's 32 that exist
         auto page_of = [&](int j) -> int {
             const int pos = g.k0 + j * TKT + warp * 32 + lane;
             if (pos < cur.t.lo || pos >= cur.t.hi) return -1;
@@ -263,17 +281,17 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             int j;   // K0 (K1) | V0 K(a) | V1 K(a+1) | ... | the last V
             if (r < 0) is_v = false, j = idx;
             else if (r < 2 * both) is_v = !(r & 1), j = (r >> 1) + (r & 1 ? a : 0);
-            else is_v = true, j = both + r - 2 * both;
+            else is_v = true, j = r - both;
+            tile_no = tile_base + j;
             if (idx == 0) page_next = page_of(0);
             if (!is_v) {
-                const int pos = g.k0 + j * TKT + warp * 32 + lane;
                 uint32_t off = ~0u;
                 int sp = 0;
                 if (page_next >= c.n_pages) {
                     atomicCAS(p.err, 0, KERR_PAGE);
                 } else if (page_next >= 0) {
                     int ip, slot;
-                    paged_split(p, pos, ip, slot);
+                    paged_split(p, g.k0 + j * TKT + warp * 32 + lane, ip, slot);
                     off = (uint32_t)((page_next * c.stride[0] + slot * c.stride[1] + cur.h * c.stride[2]) * T::ES >> 4);
                     if constexpr (T::Q8) sp = (int)(page_next * c.scale_stride[0] + slot * c.scale_stride[1] + cur.h * c.scale_stride[2]);
                 }
@@ -283,68 +301,55 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             }
             off_now = j & 1 ? off1 : off0;
             sp_now = j & 1 ? sp1 : sp0;
-            const uint32_t live = __ballot_sync(0xffffffffu, off_now != ~0u);
-            bool mixed = false;
-            if constexpr (T::DIRECT) {   // does every row of the item see all of this tile?
+            live = __ballot_sync(0xffffffffu, off_now != ~0u);
+            if constexpr (T::DIRECT) {   // do rows of the item see this tile differently?
                 const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = cur.s.L - cur.s.n, k = g.k0 + j * TKT;
                 mixed = is_v && tok1 > tok0 && ((p.a.causal && k + TKT > at0 + tok0 + 1) || (p.a.window > 0 && k < at0 + tok1 - p.a.window + 1));
             }
-            if (lane == 0) {
-                meta[n_copy & 7] = (is_v ? 1u : 0u) | (mixed ? 2u : 0u) | (uint32_t)(tile_base + j) << 2;
-                there[n_copy & 7] = live;
+        };
+        auto end_load = [&]() {
+            n_copy++;
+            if (++idx == 2 * g.tiles) {
+                idx = 0;
+                tile_base += g.tiles;
+                u += g.tiles;
+                cur.next_item<T::R>(p);
+                if (u < u_end) g = segment_of<T>(p, cur, u, u_end);
             }
         };
-        auto copy_piece = [&]() {
-            if (part == 0) begin_load();
-            uint32_t dst;
-            if constexpr (T::DIRECT) {
-                const int s = n_copy % T::SLOTS;
-                if (n_copy >= T::SLOTS)
-                    ok = wait_warp(&bar.empty[s], (n_copy / T::SLOTS - 1) & 1, abort_flag, p.err, ERR_P_LOAD);
-                if (!ok) return;
-                dst = ring + (uint32_t)s * T::SLOT;
-            } else {
-                dst = raw + (uint32_t)((n_copy * PIECES + part) % T::NRAW) * T::RAW_PIECE;
-            }
-            const uint8_t* base = static_cast<const uint8_t*>(is_v ? c.v : c.k);
+        // Rows i0 .. i0 + N - 1 (of the warp's loads) to to(i).
+        auto copy_rows = [&](int i0, auto to) {
+            const uint8_t* base = is_v ? v_lane : k_lane;
+            if (live == 0xffffffffu) {
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                const int r = (part * PER + i) * ROWS + sub_row;
-                const uint32_t o = __shfl_sync(0xffffffffu, off_now, r);
-                const uint8_t* src = base + ((uint64_t)(o == ~0u ? 0 : o) << 4) + piece16 * 16;
-                cp_async16(T::DIRECT ? dst + tile_at(warp * 32 + r, piece16 * 16) : dst + i * 2048, src, o != ~0u);
-            }
-            if constexpr (T::Q8)
-                if (part == 0)
-                    cp_async4(ptx::smem_u32(smem + T::OFF_RAW_SCALE) + ((n_copy & 7) * 128 + tid) * 4, (is_v ? c.v_scale : c.k_scale) + sp_now,
-                              off_now != ~0u);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (++part == PIECES) {
-                part = 0;
-                n_copy++;
-                if (++idx == 2 * g.tiles) {
-                    idx = 0;
-                    tile_base += g.tiles;
-                    u += g.tiles;
-                    cur.next_item<T::R, TKT>(p);
-                    if (u < u_end) g = segment_of<T>(p, cur, u, u_end);
+                for (int i = 0; i < PER; i++) {
+                    const uint32_t o = __shfl_sync(0xffffffffu, off_now, (i0 + i) * ROWS + sub_row);
+                    cp_async16(to(i), base + ((uint64_t)o << 4));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    const uint32_t o = __shfl_sync(0xffffffffu, off_now, (i0 + i) * ROWS + sub_row);
+                    cp_async16(to(i), o == ~0u ? base : base + ((uint64_t)o << 4), o != ~0u);
                 }
             }
         };
-        // ---- handing over ----
-        int n_done = 0, done_part = 0;
-        uint32_t top_all = 0;   // own scales: the largest of this lane's rows (bits)
-        auto hand_piece = [&]() {
-            const uint32_t what = meta[n_done & 7], live = there[n_done & 7];
-            const bool v = what & 1;
-            const int tile_no = (int)(what >> 2), s = n_done % T::SLOTS;
-            const uint32_t dst = ring + (uint32_t)s * T::SLOT;
-            if (!v && done_part == 0 && lane == 0) bar.ok[tile_no & 7][warp] = live;
-            if constexpr (T::DIRECT) {
-                if (v && warp == 0 && lane < 4) bar.strange[(tile_no + 4) & 7][lane] = 0;   // four tiles ahead of its use
-                if (what & 2) {
+
+        if constexpr (T::DIRECT) {
+            while (ok && u < u_end) {
+                begin_load();
+                const int s = n_copy % T::SLOTS;
+                const uint32_t dst = ring + (uint32_t)s * T::SLOT;
+                if (n_copy >= T::SLOTS)
+                    ok = wait_warp(&bar.empty[s], (n_copy / T::SLOTS - 1) & 1, abort_flag, p.err, ERR_P_LOAD);
+                if (!ok) break;
+                copy_rows(0, [&](int i) { return dst + place_of(i); });
+                if (is_v && warp == 0 && lane < 4) bar.strange[(tile_no + 4) & 7][lane] = 0;   // four tiles ahead of its use
+                if (mixed) {
                     // Rows of the item see this tile differently: values that are not finite
                     // leave it (0 times them is not 0) and their positions are noted.
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    cp_wait<0>();
 #pragma unroll 1
                     for (int i = 0; i < LOADS; i++) {
                         const int r = warp * 32 + i * ROWS + sub_row;
@@ -362,11 +367,57 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                             atomicOr(&bar.strange[tile_no & 7][r >> 5], 1u << (r & 31));
                         }
                     }
+                    ptx::fence_proxy_async_smem();
+                    ptx::mbar_arrive(&bar.full[s]);
+                } else {
+                    cp_async_arrive(&bar.full[s]);       // when this thread's copies so far have landed
                 }
-            } else {
-                float* scales = v ? reinterpret_cast<float*>(smem + T::OFF_VS) + tile_no % T::VSD * 128
-                                  : reinterpret_cast<float*>(smem + T::OFF_KS) + tile_no % T::KSD * 128;
+                if (!is_v && lane == 0) bar.ok[tile_no & 7][warp] = live;
+                if (lane == 0) ptx::mbar_arrive(&bar.full[s]);   // the notes
+                if (is_v) ptx::mbar_arrive(&bar.v_notes[tile_no & 3]);
+                end_load();
+            }
+            cp_wait<0>();
+        } else {
+            constexpr int AHEAD = T::NRAW - 1;
+            volatile uint32_t* meta = bar.meta[warp];       // by load & 7: is_v | tile << 1
+            volatile uint32_t* there = bar.there[warp];
+            int part = 0, raw_c = 0;                        // piece of the load, raw slot
+            auto copy_piece = [&]() {
+                if (part == 0) {
+                    begin_load();
+                    if (lane == 0) {
+                        meta[n_copy & 7] = (is_v ? 1u : 0u) | (uint32_t)tile_no << 1;
+                        there[n_copy & 7] = live;
+                    }
+                    if constexpr (T::Q8)
+                        cp_async4(ptx::smem_u32(smem + T::OFF_RAW_SCALE) + ((n_copy & 7) * 128 + tid) * 4, (is_v ? c.v_scale : c.k_scale) + sp_now,
+                                  off_now != ~0u);
+                }
+                const uint32_t dst = raw + (uint32_t)raw_c * T::RAW_PIECE;
+                copy_rows(part * PER, [&](int i) { return dst + i * 2048; });
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                raw_c = raw_c + 1 == T::NRAW ? 0 : raw_c + 1;
+                if (++part == PIECES) {
+                    part = 0;
+                    end_load();
+                }
+            };
+            // ---- handing over ----
+            int n_done = 0, done_part = 0, raw_d = 0;
+            uint32_t top_all = 0;   // own scales: the largest of this lane's rows (bits)
+            auto hand_piece = [&]() {
+                const uint32_t what = meta[n_done & 7];
+                const bool v = what & 1;
+                const int tile = (int)(what >> 1), s = n_done % T::SLOTS;
+                const uint32_t dst = ring + (uint32_t)s * T::SLOT, src = raw + (uint32_t)raw_d * T::RAW_PIECE;
+                float* scales = v ? reinterpret_cast<float*>(smem + T::OFF_VS) + tile % (T::DIRECT ? 1 : T::VSD) * 128
+                                  : reinterpret_cast<float*>(smem + T::OFF_KS) + tile % (T::DIRECT ? 1 : T::KSD) * 128;
+                uint32_t w[PER][4];   // all of the piece at once: the conversions of its rows overlap
+#pragma unroll
+                for (int i = 0; i < PER; i++) ld_shared16(src + i * 2048, w[i]);
                 if (done_part == 0) {
+                    if (!v && lane == 0) bar.ok[tile & 7][warp] = there[n_done & 7];
                     if (n_done >= T::SLOTS)
                         ok = wait_warp(&bar.empty[s], (n_done / T::SLOTS - 1) & 1, abort_flag, p.err, ERR_P_LOAD);
                     if (!ok) return;
@@ -377,51 +428,61 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         if (scale > 0.0f && scale < INFINITY) top_all = __float_as_uint(scale);
                     }
                 }
-                const uint32_t src = raw + (uint32_t)((n_done * PIECES + done_part) % T::NRAW) * T::RAW_PIECE;
+                if constexpr (T::Q8) {
 #pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const int r = warp * 32 + (done_part * PER + i) * ROWS + sub_row;
-                    uint32_t w[4];
-                    ld_shared16(src + i * 2048, w);
-                    if constexpr (T::Q8) {
+                    for (int i = 0; i < PER; i++) {
                         uint32_t h[8];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) codes_f16<CT>(w[k], h[2 * k], h[2 * k + 1]);
-                        st_shared16(dst + tile_at(r, piece16 * 32), h[0], h[1], h[2], h[3]);
-                        st_shared16(dst + tile_at(r, piece16 * 32 + 16), h[4], h[5], h[6], h[7]);
-                    } else {
-                        constexpr int N = 16 / T::ES;
+                        for (int k = 0; k < 4; k++) codes_f16<CT>(w[i][k], h[2 * k], h[2 * k + 1]);
+                        // (the two halves of 32 bytes are neighbours up to the swizzle's lowest bit)
+                        const uint32_t at = dst + place_of(done_part * PER + i);
+                        st_shared16(at, h[0], h[1], h[2], h[3]);
+                        st_shared16(at ^ 16u, h[4], h[5], h[6], h[7]);
+                    }
+                } else {
+                    constexpr int N = 16 / T::ES;
+                    uint32_t top[PER];   // over the bits of |x|: what is not finite comes out on top
+#pragma unroll
+                    for (int i = 0; i < PER; i++) {
+                        top[i] = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            top[i] = CT == RT_BF16 ? max(top[i], max(w[i][k] << 16 & 0x7fffffffu, w[i][k] & 0x7fff0000u)) : max(top[i], w[i][k] & 0x7fffffffu);
+                    }
+#pragma unroll
+                    for (int o = LANES / 2; o; o >>= 1)
+#pragma unroll
+                        for (int i = 0; i < PER; i++) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+                    for (int i = 0; i < PER; i++) {
+                        const int at_row = done_part * PER + i, r = warp * 32 + at_row * ROWS + sub_row;
+                        const int e = f16_scale_exp(__uint_as_float(top[i]));
+                        const bool finite = top[i] < 0x7f800000u;
+                        const float up = finite ? pow2i(e) : 0.0f;
+                        const float down = finite ? pow2i(-e) : __uint_as_float(0x7fc00000u);
                         float x[N];
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             if constexpr (CT == RT_BF16) {
-                                x[2 * k] = __uint_as_float(w[k] << 16);
-                                x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+                                x[2 * k] = __uint_as_float(w[i][k] << 16) * up;
+                                x[2 * k + 1] = __uint_as_float(w[i][k] & 0xffff0000u) * up;
                             } else {
-                                x[k] = __uint_as_float(w[k]);
+                                x[k] = __uint_as_float(w[i][k]) * up;
                             }
                         }
-                        uint32_t top = 0;   // over the bits of |x|: what is not finite comes out on top
+                        if (!finite) {
 #pragma unroll
-                        for (int k = 0; k < N; k++) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
-#pragma unroll
-                        for (int o = LANES / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        const int e = f16_scale_exp(__uint_as_float(top));
-                        const bool finite = top < 0x7f800000u;
-                        const float up = finite ? pow2i(e) : 0.0f;
-                        const float down = finite ? pow2i(-e) : __uint_as_float(0x7fc00000u);
-#pragma unroll
-                        for (int k = 0; k < N; k++) x[k] = finite ? x[k] * up : 0.0f;
+                            for (int k = 0; k < N; k++) x[k] = 0.0f;
+                        }
                         if (piece16 == 0) scales[r] = down;
-                        if (finite && top) top_all = max(top_all, __float_as_uint(down));
+                        if (finite && top[i]) top_all = max(top_all, __float_as_uint(down));
+                        const uint32_t at = dst + place_of(at_row);
                         if constexpr (T::VP == 1) {
-                            st_shared16(dst + tile_at(r, piece16 * 16), f16x2_rn(x[0], x[1]), f16x2_rn(x[2], x[3]),
-                                        f16x2_rn(x[4 % N], x[5 % N]), f16x2_rn(x[6 % N], x[7 % N]));
+                            st_shared16(at, f16x2_rn(x[0], x[1]), f16x2_rn(x[2], x[3]), f16x2_rn(x[4 % N], x[5 % N]), f16x2_rn(x[6 % N], x[7 % N]));
                         } else {
                             float h[4];
 #pragma unroll
                             for (int k = 0; k < 4; k++) h[k] = round11(x[k]);
-                            const uint32_t at = dst + tile_at(r, piece16 * 8);
                             st_shared8(at, f16x2_rn(h[0], h[1]), f16x2_rn(h[2], h[3]));
                             st_shared8(at + T::PLANE, f16x2_rn(x[0] - h[0], x[1] - h[1]), f16x2_rn(x[2] - h[2], x[3] - h[3]));
                         }
@@ -429,31 +490,31 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 }
                 if (v && done_part == PIECES - 1) {
                     const uint32_t top = __reduce_max_sync(0xffffffffu, top_all);
-                    if (lane == 0) bar.vmax[tile_no & 3][warp] = __uint_as_float(top);
+                    if (lane == 0) bar.vmax[tile & 3][warp] = __uint_as_float(top);
+                }
+                raw_d = raw_d + 1 == T::NRAW ? 0 : raw_d + 1;
+                if (++done_part == PIECES) {
+                    done_part = 0;
+                    ptx::fence_proxy_async_smem();
+                    ptx::mbar_arrive(&bar.full[s]);
+                    if (v) ptx::mbar_arrive(&bar.v_notes[tile & 3]);
+                    n_done++;
+                }
+            };
+            int ahead = 0;
+            while (ok && u < u_end) {
+                copy_piece();
+                if (++ahead > AHEAD) {
+                    cp_wait<AHEAD>();
+                    __syncwarp();
+                    hand_piece();
+                    ahead--;
                 }
             }
-            if (++done_part == PIECES) {
-                done_part = 0;
-                ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive(&bar.full[s]);
-                if (v) ptx::mbar_arrive(&bar.v_notes[tile_no & 3]);
-                n_done++;
-            }
-        };
-        int ahead = 0;
-        while (ok && u < u_end) {
-            copy_piece();
-            if (!ok) break;
-            if (++ahead > AHEAD) {
-                cp_wait<AHEAD>();
-                __syncwarp();
-                hand_piece();
-                ahead--;
-            }
+            cp_wait<0>();
+            __syncwarp();
+            for (; ok && ahead > 0; ahead--) hand_piece();
         }
-        cp_wait<0>();
-        __syncwarp();
-        for (; ok && ahead > 0; ahead--) hand_piece();
     } else if (warp < 8) {
         // ------------------------------------------------ MMA issue
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_MMA));
@@ -467,6 +528,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             auto wait_load = [&](int n) {
                 if (ok) ok = ptx::wait_bounded(&bar.full[n % T::SLOTS], (n / T::SLOTS) & 1, abort_flag, p.err, ERR_P_MMA, WAIT_NS);
                 ptx::tc_fence_after();
+                if constexpr (T::DIRECT) ptx::fence_proxy_async_smem();   // the copies landed as ordinary writes
             };
             auto release = [&](int n) { ptx::mma_commit(&bar.empty[n % T::SLOTS]); };
             auto scores = [&](int chain, int q_tile, int load) {   // S = Q.K^T: all features, hi.hi then the cross terms
@@ -549,7 +611,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                     }
                 }
                 u += g.tiles;
-                cur.next_item<T::R, TKT>(p);
+                cur.next_item<T::R>(p);
             }
             ptx::mma_commit(&bar.drain);   // nothing in flight when TMEM is given back
             volatile int no_abort = 0;
@@ -990,7 +1052,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             }
             tile_base += g.tiles;
             u += g.tiles;
-            cur.next_item<T::R, TKT>(p);
+            cur.next_item<T::R>(p);
         }
     }
     __syncthreads();
@@ -1018,12 +1080,15 @@ Status tiles_as(PagedArgs& p, void* ws, cudaStream_t st) {
     static const cudaError_t set = cudaFuncSetAttribute(paged_tiles_kernel<CT, F32ACT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
     RT_CUDA_CHECK(set);
     const int blocks = tiles_blocks(p.a);
-    p.part = static_cast<float*>(ws);
+    paged_set_workspace(p, ws, blocks);
     p.whole = 0;
+    p.key_shift = 7;
+    p.head_group = 1;
+    p.head_groups = p.a.cache.n_heads;
     p.min_units = MIN_UNITS;
     paged_tiles_kernel<CT, F32ACT, D><<<blocks, TT, T::SMEM, st>>>(p);
     RT_LAUNCH_CHECK();
-    return blocks == 1 ? Status::ok() : launch_paged_join<D, T::R, TKT>(p, blocks, st);
+    return blocks == 1 ? Status::ok() : launch_paged_join<D, T::R>(p, blocks, st);
 }
 template <int CT, bool F32ACT>
 Status tiles_dim(PagedArgs& p, void* ws, cudaStream_t st) {
@@ -1036,7 +1101,7 @@ bool paged_tiles_takes(const RtPagedAttention& p) { return p.cache.head_dim == 6
 
 size_t paged_tiles_workspace(const RtPagedAttention& p) {
     const int R = tile_rows(p);
-    return (size_t)tiles_blocks(p) * 2 * (R * p.cache.head_dim + 2 * R) * sizeof(float);
+    return paged_workspace(tiles_blocks(p), 1, R * p.cache.head_dim + 2 * R);
 }
 
 Status launch_paged_tiles(PagedArgs& p, void* ws, cudaStream_t st) {

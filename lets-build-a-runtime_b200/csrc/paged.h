@@ -3,8 +3,8 @@
 //
 // The rows of a sequence are its (new token, query head of a cache head)
 // pairs, token-major, cut into tiles of R rows; an item is one row tile of one
-// sequence and cache head, and its units are the key tiles of KT positions
-// that at least one of its rows sees.  Lengths are known on the device only,
+// sequence and one group of cache heads, and its units are the key tiles of 2^key_shift
+// positions that at least one of its rows sees.  Lengths are known on the device only,
 // so every block derives the same list from them: sequences in order, then row
 // tiles, cache heads, key tiles.  Block c takes units [c * per, (c + 1) * per)
 // of the whole list, so blocks finish together however unequal the sequences
@@ -19,16 +19,29 @@
 
 namespace rt {
 
+struct PagedNote;
 struct PagedArgs {
     RtPagedAttention a;
-    float* part;       // [2 * blocks][R * DP + 2 * R]: sums, maxima (log2 units), weight sums
+    float* part;       // [2 * blocks][heads of a group][R * DP + 2 * R]: sums, maxima (log2 units), weight sums
+    PagedNote* notes;  // per block: the item to be joined there
     int* err;
     int group;         // query heads per cache head
     int whole;         // 1: a block takes whole items (no join)
     int min_units;
+    int key_shift;     // log2 of the positions of a key tile
+    int head_group;    // cache heads of an item
+    int head_groups;
     int page_shift;    // log2 of the page size, -1 when it is not a power of two
     bool vec_q, vec_out;   // every row of q / out starts on 16 bytes
 };
+// Workspace: the notes, then the slots.
+inline size_t paged_workspace(int blocks, int head_group, int slot_floats) {
+    return (((size_t)blocks * 32 + 255) & ~(size_t)255) + (size_t)blocks * 2 * head_group * slot_floats * sizeof(float);
+}
+inline void paged_set_workspace(PagedArgs& p, void* ws, int blocks) {
+    p.notes = static_cast<PagedNote*>(ws);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + (((size_t)blocks * 32 + 255) & ~(size_t)255));
+}
 inline bool paged_rows16(const void* p, const int64_t st[2], int dtype) {
     return aligned16(p) && (st[0] * dtype_bytes(dtype)) % 16 == 0 && (st[1] * dtype_bytes(dtype)) % 16 == 0;
 }
@@ -60,15 +73,15 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& p, int b) {
     return s;
 }
 
-template <int R, int KT>
+template <int R>
 __device__ __forceinline__ PagedTiles paged_tiles(const PagedArgs& p, const PagedSeq& s, int qt) {
     PagedTiles t;
     const int last = (min((qt + 1) * R, s.n * p.group) - 1) / p.group, first = qt * R / p.group;
     t.hi = p.a.causal ? min(s.L, s.L - s.n + last + 1) : s.L;
     t.lo = p.a.window > 0 ? max(0, s.L - s.n + first - p.a.window + 1) : 0;
     if (t.lo >= t.hi) t.lo = t.hi = 0;
-    t.t0 = t.lo / KT;
-    t.count = max(1, (t.hi + KT - 1) / KT - t.t0);
+    t.t0 = t.lo >> p.key_shift;
+    t.count = max(1, ((t.hi + (1 << p.key_shift) - 1) >> p.key_shift) - t.t0);
     return t;
 }
 
@@ -77,15 +90,15 @@ __device__ __forceinline__ int paged_row_tiles(const PagedArgs& p, const PagedSe
     return (int)(((int64_t)s.n * p.group + R - 1) / R);
 }
 
-template <int R, int KT>
+template <int R>
 __device__ __forceinline__ int paged_units(const PagedArgs& p, int b) {
     if (b >= p.a.n_seqs) return 0;
     const PagedSeq s = paged_seq(p, b);
     const int nq = paged_row_tiles<R>(p, s);
-    if (p.whole) return nq * p.a.cache.n_heads;
+    if (p.whole) return nq * p.head_groups;
     int sum = 0;
-    for (int q = 0; q < nq; q++) sum += paged_tiles<R, KT>(p, s, q).count;
-    return sum * p.a.cache.n_heads;
+    for (int q = 0; q < nq; q++) sum += paged_tiles<R>(p, s, q).count;
+    return sum * p.head_groups;
 }
 
 // Inclusive sum over the block's T threads; `total` gets the block's sum.
@@ -114,9 +127,9 @@ __device__ __forceinline__ int paged_scan(int x, int* sh, int* total) {
 struct PagedCursor {
     PagedSeq s;
     PagedTiles t;
-    int nq, qt, h, i;     // row tiles of the sequence; row tile, cache head, key tile inside the item
+    int nq, qt, h, i;     // row tiles of the sequence; row tile, head group, key tile inside the item
 
-    template <int R, int KT>
+    template <int R>
     __device__ __forceinline__ void open(const PagedArgs& p, int b) {   // the first item at or after sequence b
         qt = h = i = 0;
         nq = 0;
@@ -127,29 +140,29 @@ struct PagedCursor {
             if (nq > 0) break;
             s.b++;
         }
-        if (nq > 0) t = paged_tiles<R, KT>(p, s, 0);
+        if (nq > 0) t = paged_tiles<R>(p, s, 0);
     }
-    template <int R, int KT>
+    template <int R>
     __device__ __forceinline__ void next_item(const PagedArgs& p) {
         i = 0;
-        if (++h < p.a.cache.n_heads) return;
+        if (++h < p.head_groups) return;
         h = 0;
-        if (++qt < nq) t = paged_tiles<R, KT>(p, s, qt);
-        else open<R, KT>(p, s.b + 1);
+        if (++qt < nq) t = paged_tiles<R>(p, s, qt);
+        else open<R>(p, s.b + 1);
     }
 };
 
 // The units of this call and the block's share.  `unit`: the first unit to
 // look at (c * per).  False when the block has none.  sh: T / 32 + 2 ints.
-template <int T, int R, int KT>
+template <int T, int R>
 __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, int blocks, int* sh, PagedCursor& c, int& u,
                                                int& per, int& total) {
-    int mine = paged_units<R, KT>(p, threadIdx.x), all;
+    int mine = paged_units<R>(p, threadIdx.x), all;
     int incl = paged_scan<T>(mine, sh, &all);
     total = all;
     for (int base = T; base < p.a.n_seqs; base += T) {
         int part;
-        paged_scan<T>(paged_units<R, KT>(p, base + threadIdx.x), sh, &part);
+        paged_scan<T>(paged_units<R>(p, base + threadIdx.x), sh, &part);
         total += part;
     }
     per = max(p.min_units, (total + blocks - 1) / blocks);
@@ -158,7 +171,7 @@ __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, in
     int carry = 0;
     for (int base = 0;; base += T) {
         if (base) {
-            mine = paged_units<R, KT>(p, base + threadIdx.x);
+            mine = paged_units<R>(p, base + threadIdx.x);
             incl = paged_scan<T>(mine, sh, &all);
         }
         const int first = carry + incl - mine;
@@ -173,16 +186,16 @@ __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, in
     const int b = sh[T / 32];
     int r = u - sh[T / 32 + 1];
     __syncthreads();
-    c.open<R, KT>(p, b);
+    c.open<R>(p, b);
     while (true) {   // row tile, then head and key tile
-        const int per_head = p.whole ? 1 : c.t.count, n = per_head * p.a.cache.n_heads;
+        const int per_head = p.whole ? 1 : c.t.count, n = per_head * p.head_groups;
         if (r < n) {
             c.h = r / per_head;
             c.i = r % per_head;
             return true;
         }
         r -= n;
-        c.t = paged_tiles<R, KT>(p, c.s, ++c.qt);
+        c.t = paged_tiles<R>(p, c.s, ++c.qt);
     }
 }
 
@@ -240,58 +253,128 @@ __device__ __forceinline__ void paged_store_lse(const PagedArgs& p, const PagedS
             l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// Adds up the items that fell into several blocks: block (c, y) looks at the
-// boundary between blocks c and c + 1 of the main kernel, and takes rows
-// 16 y .. of the item.  Started early (its own schedule overlaps the main
-// kernel's tail), it waits for the main kernel before it reads.
-constexpr int JOIN_ROWS = 16, JOIN_THREADS = 128;
-template <int DP, int R, int KT>
+// A block that starts inside an item leaves a note for the join kernel if it is
+// the first one to do so: what is to be added up there.  Every block writes one.
+struct PagedNote {
+    int first, n, L, b;        // the sequence
+    int qt, h, from, count;    // row tile, head group; blocks the item lies in
+};
+template <int R>
+__device__ __forceinline__ void paged_note(const PagedArgs& p, bool some, const PagedCursor& c, int u, int per) {
+    if (p.whole || threadIdx.x) return;
+    PagedNote x = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (some && c.i > 0) {
+        const int first = u - c.i, from = first / per;
+        if (from == (int)blockIdx.x - 1) x = {c.s.first, c.s.n, c.s.L, c.s.b, c.qt, c.h, from, (first + c.t.count - 1) / per - from + 1};
+    }
+    p.notes[blockIdx.x] = x;
+}
+
+// Adds up the items that fell into several blocks: block (c, y, z) takes what
+// block c + 1 of the main kernel noted, some rows of the item, head z of its
+// group.  An item of a long sequence may lie in hundreds of blocks: their
+// maxima are read side by side, and the sums by several threads per feature,
+// each with several loads under way; the order of additions is fixed.
+constexpr int JOIN_THREADS = 256;
+template <int DP, int R>
+struct Join {
+    static constexpr int ROWS = R <= 32 ? R / 4 : 16;                  // rows of a block
+    static constexpr int ITEMS = ROWS * DP / 4;                        // 4 features of a row each
+    static constexpr int PARTS = ITEMS >= JOIN_THREADS ? 1 : JOIN_THREADS / ITEMS;   // threads that share an item
+};
+template <int DP, int R>
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_constant__ PagedArgs p, int blocks) {
-    __shared__ int sched[JOIN_THREADS / 32 + 2];
-    PagedCursor cur;
-    int u, per, total;
-    const bool some = paged_schedule<JOIN_THREADS, R, KT>(p, blockIdx.x + 1, blocks, sched, cur, u, per, total);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!some || cur.i == 0) return;
-    const int first = u - cur.i, c0 = blockIdx.x;
-    if (first < c0 * per) return;                          // an earlier boundary lies in this item
-    const int c1 = (first + cur.t.count - 1) / per;
+    using J = Join<DP, R>;
+    __shared__ float top[J::ROWS][JOIN_THREADS / J::ROWS], sums[J::PARTS > 1 ? JOIN_THREADS : 1][4];
+    extern __shared__ float factor[];                      // [blocks of the item][ROWS]
+    asm volatile("griddepcontrol.wait;" ::: "memory");     // (launched while the main kernel runs)
+    const PagedNote note = p.notes[blockIdx.x + 1];
+    if (note.count == 0) return;
+    const int c0 = note.from, n = note.count;
     constexpr int SLOT = R * DP + 2 * R;
-    const PagedSeq& s = cur.s;
-    const int row0 = cur.qt * R, rows = min(R, s.n * p.group - row0);
-    for (int e = threadIdx.x; e < JOIN_ROWS * DP / 4; e += JOIN_THREADS) {
-        const int r = blockIdx.y * JOIN_ROWS + e / (DP / 4), d = e % (DP / 4) * 4;
-        if (r >= rows) return;
+    const int z = blockIdx.z, h = note.h * p.head_group + z;
+    auto slot_of = [&](int k) { return p.part + ((int64_t)(2 * (c0 + k) + (k == 0)) * p.head_group + z) * SLOT; };
+    const PagedSeq s = {note.b, note.first, note.n, note.L};
+    const int row0 = note.qt * R, rows = min(R, s.n * p.group - row0);
+    for (int first_row = blockIdx.y * J::ROWS; first_row < rows; first_row += gridDim.y * J::ROWS) {
+        __syncthreads();
+        // ---- the rows' maxima and weight sums ----
+        const int tid = threadIdx.x, lr = tid % J::ROWS, lane = tid / J::ROWS;
+        constexpr int LANES = JOIN_THREADS / J::ROWS;
+        const bool mine = first_row + lr < rows;
         float m = -INFINITY;
-        for (int c = c0; c <= c1; c++) m = fmaxf(m, p.part[(int64_t)(2 * c + (c == c0)) * SLOT + R * DP + r]);
-        float sum[4] = {0, 0, 0, 0}, ls = 0.0f;
-        if (m != -INFINITY)
-#pragma unroll 4
-            for (int c = c0; c <= c1; c++) {
-                const float* part = p.part + (int64_t)(2 * c + (c == c0)) * SLOT;
-                const float f = exp2_fast(part[R * DP + r] - m);
-                if (f == 0.0f) continue;
-                const float4 x = *reinterpret_cast<const float4*>(part + r * DP + d);
-                sum[0] += x.x * f; sum[1] += x.y * f; sum[2] += x.z * f; sum[3] += x.w * f;
-                ls += part[R * DP + R + r] * f;
+        if (mine)
+            for (int k = lane; k < n; k += LANES) {
+                const float x = slot_of(k)[R * DP + first_row + lr];
+                factor[k * J::ROWS + lr] = x;
+                m = fmaxf(m, x);
             }
-        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-        if (d < p.a.cache.head_dim) paged_store4(p, s, cur.h, row0 + r, d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
-        if (d == 0) paged_store_lse(p, s, cur.h, row0 + r, m, ls);
+        top[lr][lane] = m;
+        __syncthreads();
+        for (int k = 0; k < LANES; k++) m = fmaxf(m, top[lr][k]);
+        __syncthreads();
+        float ls = 0.0f;
+        if (mine)
+            for (int k = lane; k < n; k += LANES) {
+                const float x = factor[k * J::ROWS + lr], f = x == -INFINITY ? 0.0f : exp2_fast(x - m);
+                factor[k * J::ROWS + lr] = f;
+                ls += f == 0.0f ? 0.0f : slot_of(k)[R * DP + R + first_row + lr] * f;
+            }
+        top[lr][lane] = ls;
+        __syncthreads();
+        ls = 0.0f;
+        for (int k = 0; k < LANES; k++) ls += top[lr][k];
+        if (mine && lane == 0) paged_store_lse(p, s, h, row0 + first_row + lr, m, ls);
+        __syncthreads();
+        if (lane == 0) top[lr][0] = ls == 0.0f ? 0.0f : 1.0f / ls;
+        __syncthreads();
+        // ---- the sums ----
+        for (int e0 = 0; e0 < J::ITEMS; e0 += JOIN_THREADS) {
+            const int e = e0 + tid % (JOIN_THREADS / J::PARTS), part = tid / (JOIN_THREADS / J::PARTS);
+            const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+            float sum[4] = {0, 0, 0, 0};
+            if (first_row + r < rows) {
+#pragma unroll 8
+                for (int k = part; k < n; k += J::PARTS) {
+                    const float f = factor[k * J::ROWS + r];
+                    const float4 x = f == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(slot_of(k) + (first_row + r) * DP + d);
+                    sum[0] += x.x * f; sum[1] += x.y * f; sum[2] += x.z * f; sum[3] += x.w * f;
+                }
+            }
+            if constexpr (J::PARTS > 1) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) sums[tid][j] = sum[j];
+                __syncthreads();
+                if (part == 0) {
+#pragma unroll
+                    for (int k = 1; k < J::PARTS; k++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) sum[j] += sums[tid + k * (JOIN_THREADS / J::PARTS)][j];
+                }
+            }
+            if (part == 0 && first_row + r < rows && d < p.a.cache.head_dim) {
+                const float inv = top[r][0];
+                paged_store4(p, s, h, row0 + first_row + r, d, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+            }
+        }
     }
 }
-template <int DP, int R, int KT>
+template <int DP, int R>
 Status launch_paged_join(const PagedArgs& p, int blocks, cudaStream_t st) {
+    using J = Join<DP, R>;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks - 1, (R + JOIN_ROWS - 1) / JOIN_ROWS);
+    const int64_t most = (int64_t)(p.a.max_new < p.a.total_new ? p.a.max_new : p.a.total_new) * p.group;   // (a bound of the host's: blocks loop)
+    const int tall = (int)(most < 1 ? 1 : most < R ? most : R);
+    cfg.gridDim = dim3(blocks - 1, (tall + J::ROWS - 1) / J::ROWS, p.head_group);
     cfg.blockDim = dim3(JOIN_THREADS);
+    cfg.dynamicSmemBytes = (size_t)blocks * J::ROWS * sizeof(float);   // an item in every block at most
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_join_kernel<DP, R, KT>, p, blocks));
+    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_join_kernel<DP, R>, p, blocks));
     return Status::ok();
 }
 #endif
