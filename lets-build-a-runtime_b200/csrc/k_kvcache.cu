@@ -7,7 +7,10 @@
 // fp32 or 8 bf16 features), so dense loads and stores of neighbouring lanes
 // join into whole lines and a row's maximum is a few shuffles.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+#include <algorithm>
 
 #include "rt_internal.h"
 
@@ -97,177 +100,240 @@ __device__ __forceinline__ void put_cache(void* base, int64_t off, const float (
         else *p = w[0];
     }
 }
+// The same the other way, in two steps: the loads of several rows go first.
 template <int N, int CT>
-__device__ __forceinline__ void get_cache(const void* base, int64_t off, float (&x)[N]) {
-    if constexpr (CT == RT_F32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + off);
+struct Raw {
+    static constexpr int WORDS = CT == RT_F32 ? N : CT == RT_BF16 ? N / 2 : N / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const float4 v = p[i];
-            x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
-        }
-    } else if constexpr (CT == RT_BF16) {
-        const uint2* p = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + off);
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint2 v = p[i];
-            x[4 * i] = __uint_as_float(v.x << 16);
-            x[4 * i + 1] = __uint_as_float(v.x & 0xffff0000u);
-            x[4 * i + 2] = __uint_as_float(v.y << 16);
-            x[4 * i + 3] = __uint_as_float(v.y & 0xffff0000u);
-        }
-    } else {
-        uint32_t w[N / 4];
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) + off);
-        if constexpr (N == 8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            w[0] = v.x; w[1] = v.y;
-        } else {
-            w[0] = *p;
-        }
-#pragma unroll
-        for (int i = 0; i < N / 4; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (CT == RT_I8) {
-                    x[4 * i + j] = (float)(int8_t)(w[i] >> (8 * j));
-                } else {
-                    __nv_fp8_e4m3 v;
-                    v.__x = (__nv_fp8_storage_t)(w[i] >> (8 * j));
-                    x[4 * i + j] = (float)v;
-                }
-            }
+        for (int i = 0; i < WORDS; i++) w[i] = 0;
     }
-}
-
+    __device__ __forceinline__ void load(const void* base, int64_t off) {
+        const uint8_t* p = static_cast<const uint8_t*>(base) + off * (CT == RT_F32 ? 4 : CT == RT_BF16 ? 2 : 1);
+        if constexpr (WORDS == 1) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (WORDS == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            w[0] = x.x; w[1] = x.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p + i * 4);
+                w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if constexpr (CT == RT_F32) {
+                x[i] = __uint_as_float(w[i]);
+            } else if constexpr (CT == RT_BF16) {
+                x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+            } else if constexpr (CT == RT_I8) {
+                x[i] = (float)(int8_t)(w[i / 4] >> (8 * (i & 3)));
+            } else if (i % 2 == 0) {
+                uint32_t h;
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w[i / 4] >> (8 * (i & 2)))));
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                x[i] = f.x;
+                x[i + 1] = f.y;
+            }
+        }
+    }
+};
+// A block takes threadIdx.x = part of a token's rows (K's heads, then V's; a
+// token of more than 256 parts has several blocks, blockIdx.y), threadIdx.y =
+// one of the tokens it takes side by side.  A thread has the same part of
+// every token it takes, so that what belongs to the part is worked out once.
+constexpr int KV_THREADS = 256;
 struct RowMap {
     int lanes_log2;   // lanes of a row
     int units;        // lanes of a row that hold features
-    int rows_per_token;
+    int per_token;    // lanes of a token's rows
+    int tokens;       // of a block
+    uint32_t page_mul, page_shift;   // x / page_size = (x + mulhi(x, page_mul)) >> page_shift for x < 2^31
 };
-
-template <class A, int CT>
-__global__ void __launch_bounds__(256) kv_write_kernel(RtKvWrite w, RowMap m, bool vec, int* err) {
-    constexpr int N = Unit<A>::N;
-    const RtKvCache& c = w.cache;
-    const int64_t tid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t rows = (int64_t)w.n_tokens * m.rows_per_token;
-    const int64_t row = tid >> m.lanes_log2;
-    const int unit = (int)(tid & ((1 << m.lanes_log2) - 1));
-    if (row >= rows) return;   // whole rows leave together
-    const int token = (int)(row / m.rows_per_token), r = (int)(row % m.rows_per_token);
-    const int is_v = r >= c.n_heads, head = is_v ? r - c.n_heads : r;
-    const int64_t slot = w.slots[token];
-    const bool live = unit < m.units;
-    float x[N];
-    const int64_t* st = is_v ? w.v_stride : w.k_stride;
-    const A* src = static_cast<const A*>(is_v ? w.v : w.k) + token * st[0] + head * st[1] + unit * N;
-    if (live) {
-        load_unit(src, vec, x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = 0.0f;
-    }
-    if (slot < 0) return;
-    if (slot >= (int64_t)c.n_pages * c.page_size) {
-        if (unit == 0) atomicCAS(err, 0, KERR_SLOT);
-        return;
-    }
-    const int64_t page = slot / c.page_size, off = slot % c.page_size;
-    void* dst = is_v ? c.v : c.k;
-    const int64_t at = page * c.stride[0] + off * c.stride[1] + head * c.stride[2] + unit * N;
-    if constexpr (CT == RT_I8 || CT == RT_F8E4M3) {
-        constexpr float MAX_CODE = CT == RT_I8 ? 127.0f : 448.0f;
-        // the maximum over the bits of |x|: NaN and infinity come out on top
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < N; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-        const uint32_t group = m.lanes_log2 == 5 ? 0xffffffffu
-                                                 : ((1u << (1 << m.lanes_log2)) - 1) << ((threadIdx.x & 31) >> m.lanes_log2 << m.lanes_log2);
-        top = __reduce_max_sync(group, top);
-        const float a = __uint_as_float(top);
-        // scale = a (1/M) and code = round(x ((1/a) M)), each step rounded to fp32:
-        // a function of the row that any fp32 arithmetic reproduces bit for bit
-        float scale = __fmul_rn(a, 1.0f / MAX_CODE), inv = __fmul_rn(__frcp_rn(a), MAX_CODE);
-        if (a < 7.888609052210118e-31f) scale = inv = 0.0f;                   // 2^-100: M / a overflows further down
-        if (top >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); inv = 0.0f; }
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = inv == 0.0f ? 0.0f : __fmul_rn(x[i], inv);
-        if (unit == 0)
-            (is_v ? c.v_scale : c.k_scale)[page * c.scale_stride[0] + off * c.scale_stride[1] + head * c.scale_stride[2]] = scale;
-    }
-    if (live) put_cache<N, CT>(dst, at, x);
+struct Part {
+    bool is_v, live;  // live: holds features
+    int head, unit;
+};
+__device__ __forceinline__ Part part_of(const RowMap& m, int n_heads) {
+    const int u = blockIdx.y * blockDim.x + threadIdx.x, row = u >> m.lanes_log2;
+    Part x;
+    x.unit = u & ((1 << m.lanes_log2) - 1);
+    x.is_v = row >= n_heads;
+    x.head = x.is_v ? row - n_heads : row;
+    x.live = x.unit < m.units && u < m.per_token;
+    return x;
+}
+// Where a token's slot begins in the cache and among the scales; `at` < 0: nowhere.
+struct Place {
+    int64_t at, scale;
+};
+__device__ __forceinline__ Place place_of(const RtKvCache& c, int64_t page, int off) {
+    return {page * c.stride[0] + off * c.stride[1], page * c.scale_stride[0] + off * c.scale_stride[1]};
 }
 
-// 16 tokens a block: their places in the cache are looked up once, then the
-// block's threads take the tokens' rows.
-constexpr int READ_TOKENS = 16;
+// A thread has its part of WRITE_BATCH tokens under way at a time.
+constexpr int WRITE_BATCH = 4;
 template <class A, int CT>
-__global__ void __launch_bounds__(256) kv_read_kernel(RtKvRead r, RowMap m, bool vec, int* err) {
+__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const __grid_constant__ RtKvWrite w, const __grid_constant__ RowMap m, bool vec, int* err) {
+    constexpr int N = Unit<A>::N;
+    const RtKvCache& c = w.cache;
+    const Part x = part_of(m, c.n_heads);
+    const int64_t* st = x.is_v ? w.v_stride : w.k_stride;
+    const A* src = static_cast<const A*>(x.is_v ? w.v : w.k) + x.head * st[1] + x.unit * N;
+    void* dst = x.is_v ? c.v : c.k;
+    float* scales = x.is_v ? c.v_scale : c.k_scale;
+    const int64_t at = x.head * c.stride[2] + x.unit * N, scale_at = x.head * c.scale_stride[2];
+    const int t0 = blockIdx.x * m.tokens, n = min(m.tokens, w.n_tokens - t0);
+    for (int b0 = 0; b0 < n; b0 += WRITE_BATCH * blockDim.y) {   // (all lanes of a warp alike, for the shuffles)
+        const int b = b0 + threadIdx.y;
+        float v[WRITE_BATCH][N];
+        int64_t slots[WRITE_BATCH];
+#pragma unroll
+        for (int i = 0; i < WRITE_BATCH; i++) {
+            const int token = b + i * blockDim.y;
+            slots[i] = token < n ? w.slots[t0 + token] : -1;
+            if (token < n && x.live) {
+                load_unit(src + (t0 + token) * st[0], vec, v[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++) v[i][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < WRITE_BATCH; i++) {
+            float scale = 0.0f;
+            if constexpr (CT == RT_I8 || CT == RT_F8E4M3) {
+                constexpr float MAX_CODE = CT == RT_I8 ? 127.0f : 448.0f;
+                // the maximum over the bits of |x|: NaN and infinity come out on top
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < N; j++) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+                for (int o = 1 << m.lanes_log2 >> 1; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float a = __uint_as_float(top);
+                // scale = a (1/M) and code = round(x ((1/a) M)), each step rounded to fp32:
+                // a function of the row that any fp32 arithmetic reproduces bit for bit
+                float inv = __fmul_rn(__frcp_rn(a), MAX_CODE);
+                scale = __fmul_rn(a, 1.0f / MAX_CODE);
+                if (a < 7.888609052210118e-31f) scale = inv = 0.0f;                   // 2^-100: M / a overflows further down
+                if (top >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); inv = 0.0f; }
+#pragma unroll
+                for (int j = 0; j < N; j++) v[i][j] = inv == 0.0f ? 0.0f : __fmul_rn(v[i][j], inv);
+            }
+            if (slots[i] < 0 || !x.live) continue;
+            if (slots[i] >= (int64_t)c.n_pages * c.page_size) {
+                atomicCAS(err, 0, KERR_SLOT);
+                continue;
+            }
+            const uint32_t slot = (uint32_t)slots[i], page = (slot + __umulhi(slot, m.page_mul)) >> m.page_shift;
+            const Place p = place_of(c, page, slot - page * c.page_size);
+            if constexpr (CT == RT_I8 || CT == RT_F8E4M3)
+                if (x.unit == 0) scales[p.scale + scale_at] = scale;
+            put_cache<N, CT>(dst, p.at + at, v[i]);
+        }
+    }
+}
+
+// A block looks its tokens' places up once (offsets, starts and pages are a
+// chain of loads), then its threads take them READ_BATCH at a time.
+constexpr int READ_TOKENS = 16, READ_BATCH = 8;
+template <class A, int CT>
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_constant__ RtKvRead r, const __grid_constant__ RowMap m, bool vec, int* err) {
     constexpr int N = Unit<A>::N;
     const RtKvCache& c = r.cache;
-    __shared__ int64_t place[READ_TOKENS], scale_place[READ_TOKENS];
-    const int t0 = blockIdx.x * READ_TOKENS;
-    if (threadIdx.x < READ_TOKENS) {
-        const int row = t0 + threadIdx.x;
-        int64_t p = -1, sp = 0;
-        if (row < r.n_rows && row < r.cu[r.n_seqs]) {
-            int lo = 0, hi = r.n_seqs;   // the sequence whose rows hold this one: cu[lo] <= row < cu[lo + 1]
+    __shared__ Place place[READ_TOKENS];
+    const int t0 = blockIdx.x * m.tokens, n = min(m.tokens, r.n_rows - t0);
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < n; i += blockDim.x * blockDim.y) {
+        const int row = t0 + i;
+        Place p = {-1, 0};
+        // the sequence whose rows hold this one: cu[lo] <= row < cu[lo + 1]
+        int lo = 0;
+        if (r.n_seqs <= 32) {   // their offsets side by side: one trip to memory, not one per halving
+#pragma unroll 8
+            for (int b = 1; b < r.n_seqs; b++) lo += r.cu[b] <= row;
+        } else {
+            int hi = r.n_seqs;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (r.cu[mid] <= row) lo = mid;
                 else hi = mid;
             }
-            const int64_t pos = (r.start ? r.start[lo] : 0) + (int64_t)(row - r.cu[lo]);
-            const int64_t ip = pos / c.page_size, off = pos % c.page_size;
-            if (pos < 0 || ip >= r.table_width || row < r.cu[lo]) {
+        }
+        const int first = r.cu[lo];
+        if (row < r.cu[r.n_seqs]) {
+            const int64_t pos = (r.start ? r.start[lo] : 0) + (int64_t)(row - first);
+            if (pos < 0 || pos >= min((int64_t)r.table_width * c.page_size, (int64_t)0x7fffffff) || row < first) {
                 atomicCAS(err, 0, KERR_LENGTH);
             } else {
+                const uint32_t ip = ((uint32_t)pos + __umulhi((uint32_t)pos, m.page_mul)) >> m.page_shift;
                 const int page = r.page_table[lo * r.table_stride + ip];
-                if (page < 0 || page >= c.n_pages) {
-                    atomicCAS(err, 0, KERR_PAGE);
-                } else {
-                    p = page * c.stride[0] + off * c.stride[1];
-                    sp = page * c.scale_stride[0] + off * c.scale_stride[1];
-                }
+                if (page < 0 || page >= c.n_pages) atomicCAS(err, 0, KERR_PAGE);
+                else p = place_of(c, page, (int)pos - (int)ip * c.page_size);
             }
         }
-        place[threadIdx.x] = p;
-        scale_place[threadIdx.x] = sp;
+        place[i] = p;
     }
     __syncthreads();
-    const int n_here = min(READ_TOKENS, r.n_rows - t0);
-    const int per_token = m.rows_per_token << m.lanes_log2;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n_here * per_token; i += 256) {
-        const int token = i / per_token, u = i % per_token;
-        const int row = u >> m.lanes_log2, unit = u & ((1 << m.lanes_log2) - 1);
-        if (unit >= m.units) continue;
-        const int is_v = row >= c.n_heads, head = is_v ? row - c.n_heads : row;
-        float x[N];
-        if (place[token] >= 0) {
-            get_cache<N, CT>(is_v ? c.v : c.k, place[token] + head * c.stride[2] + unit * N, x);
-            if constexpr (CT == RT_I8 || CT == RT_F8E4M3) {
-                const float s = (is_v ? c.v_scale : c.k_scale)[scale_place[token] + head * c.scale_stride[2]];
+    const Part x = part_of(m, c.n_heads);
+    if (!x.live) return;
+    const int64_t* st = x.is_v ? r.v_stride : r.k_stride;
+    A* dst = static_cast<A*>(x.is_v ? r.v_out : r.k_out) + x.head * st[1] + x.unit * N;
+    const void* src = x.is_v ? c.v : c.k;
+    const float* scales = x.is_v ? c.v_scale : c.k_scale;
+    const int64_t at = x.head * c.stride[2] + x.unit * N, scale_at = x.head * c.scale_stride[2];
+    for (int b = threadIdx.y; b < n; b += READ_BATCH * blockDim.y) {
+        Raw<N, CT> raw[READ_BATCH];
+        float s[READ_BATCH];
 #pragma unroll
-                for (int j = 0; j < N; j++) x[j] *= s;
+        for (int i = 0; i < READ_BATCH; i++) {
+            const int token = b + i * blockDim.y;
+            s[i] = 0.0f;
+            raw[i].clear();
+            if (token < n && place[token].at >= 0) {
+                raw[i].load(src, place[token].at + at);
+                if constexpr (CT == RT_I8 || CT == RT_F8E4M3) s[i] = scales[place[token].scale + scale_at];
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; j++) x[j] = 0.0f;
         }
-        const int64_t* st = is_v ? r.v_stride : r.k_stride;
-        store_unit(static_cast<A*>(is_v ? r.v_out : r.k_out) + (t0 + token) * st[0] + head * st[1] + unit * N, vec, x);
+#pragma unroll
+        for (int i = 0; i < READ_BATCH; i++) {
+            const int token = b + i * blockDim.y;
+            if (token >= n) break;
+            float y[N];
+            raw[i].values(y);
+            if constexpr (CT == RT_I8 || CT == RT_F8E4M3) {
+#pragma unroll
+                for (int j = 0; j < N; j++) y[j] *= s[i];
+            }
+            store_unit(dst + (t0 + token) * st[0], vec, y);
+        }
     }
 }
 
+// Division by the page size as a product (Granlund and Montgomery): with 2^s
+// >= d, floor(x / d) = (x + floor(x mul / 2^32)) >> s for mul = floor(2^32 (2^s -
+// d) / d) + 1; the sum fits 32 bits while x < 2^31.
 template <class A>
-RowMap row_map(const RtKvCache& c) {
+RowMap row_map(const RtKvCache& c, int n_tokens, int most, dim3& grid, dim3& block) {
     RowMap m;
     m.units = c.head_dim / Unit<A>::N;
     m.lanes_log2 = 0;
     while ((1 << m.lanes_log2) < m.units) m.lanes_log2++;
-    m.rows_per_token = 2 * c.n_heads;
+    m.per_token = (2 * c.n_heads) << m.lanes_log2;
+    const int chunks = (m.per_token + KV_THREADS - 1) / KV_THREADS;
+    const int x = chunks == 1 ? m.per_token : ((m.per_token + chunks - 1) / chunks + 31) / 32 * 32;
+    const int side = std::min(KV_THREADS / x, most);
+    // `most` tokens a block for long calls, fewer when that would leave SMs without a block
+    const int64_t fill = (int64_t)n_tokens * chunks / (2 * g_num_sms);
+    m.tokens = std::max(side, (int)std::min<int64_t>(most, fill) / side * side);
+    grid = dim3((unsigned)(((int64_t)n_tokens + m.tokens - 1) / m.tokens), chunks);
+    block = dim3(x, std::min(side, n_tokens));
+    m.page_shift = 0;
+    while (((uint64_t)1 << m.page_shift) < (uint64_t)c.page_size) m.page_shift++;
+    m.page_mul = (uint32_t)(((uint64_t)((((uint64_t)1 << m.page_shift) - c.page_size)) << 32) / c.page_size + 1);
     return m;
 }
 // Whether every row of a dense operand starts on a 16-byte boundary.
@@ -277,19 +343,21 @@ bool vector_rows(const void* p, const int64_t st[2], int dtype) {
 
 template <class A, int CT>
 Status write_as(const RtKvWrite& w, cudaStream_t st) {
-    const RowMap m = row_map<A>(w.cache);
-    const int64_t threads = ((int64_t)w.n_tokens * m.rows_per_token) << m.lanes_log2;
+    dim3 grid, block;
+    const RowMap m = row_map<A>(w.cache, w.n_tokens, 16, grid, block);
     const bool vec = vector_rows(w.k, w.k_stride, w.dtype) && vector_rows(w.v, w.v_stride, w.dtype);
-    if ((threads + 255) / 256 > 0x7fffffff) return Status::err(RT_ERR_UNSUPPORTED, "kv_write: too many rows");
-    kv_write_kernel<A, CT><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(w, m, vec, kernel_error_flag());
+    if (grid.y > 65535) return Status::err(RT_ERR_UNSUPPORTED, "kv_write: too many heads");
+    kv_write_kernel<A, CT><<<grid, block, 0, st>>>(w, m, vec, kernel_error_flag());
     RT_LAUNCH_CHECK();
     return Status::ok();
 }
 template <class A, int CT>
 Status read_as(const RtKvRead& r, cudaStream_t st) {
-    const RowMap m = row_map<A>(r.cache);
+    dim3 grid, block;
+    const RowMap m = row_map<A>(r.cache, r.n_rows, READ_TOKENS, grid, block);
     const bool vec = vector_rows(r.k_out, r.k_stride, r.dtype) && vector_rows(r.v_out, r.v_stride, r.dtype);
-    kv_read_kernel<A, CT><<<(unsigned)((r.n_rows + READ_TOKENS - 1) / READ_TOKENS), 256, 0, st>>>(r, m, vec, kernel_error_flag());
+    if (grid.y > 65535) return Status::err(RT_ERR_UNSUPPORTED, "kv_read: too many heads");
+    kv_read_kernel<A, CT><<<grid, block, 0, st>>>(r, m, vec, kernel_error_flag());
     RT_LAUNCH_CHECK();
     return Status::ok();
 }

@@ -13,8 +13,11 @@
 // its own that cp.async fills, K and V of a piece in slots of their own so that
 // all but the one in use are under way.  The order of features and of positions
 // inside a product is free, so each thread's mma.sync fragment is made of whole
-// 16-byte parts of a row: a thread copies exactly the bytes that it will use,
-// to places of its own, and reads them back without a conflict or a barrier.
+// 16-byte parts of a row, read back without a conflict or a transpose.  A copy
+// instruction takes whole rows of K (2 x 131072 positions in bf16: 236 -> 209 us
+// against threads that copy their own parts, 64 bytes of each of 8 rows);
+// for 8-bit rows of 128 bytes, with a look-up for every 4 of them, the latter
+// is the faster one (64 sequences over int8: 164 against 177 us).
 // The warps of a block take heads of the same positions (neighbours in memory)
 // when there is enough work for that, blocks of positions of one head otherwise;
 // only then is there something to add up between them, at the end of an item.
@@ -69,6 +72,8 @@ struct Few {
     static constexpr int SUBS = 32 / SB;
     static constexpr int NT = SB / 8;                                  // score tiles of 8 positions
     static constexpr int KC = DP * ES / 64;                            // 16-byte parts of a K row per thread
+    static constexpr int K_LANES = DP * ES / 16 < 32 ? DP * ES / 16 : 32, K_ROWS = 32 / K_LANES;   // of a copy
+    static constexpr bool K_PRIVATE = ES == 1;                         // a thread copies its own parts of K
     static constexpr int VB = DP * ES / 8 < 16 ? DP * ES / 8 : 16;     // bytes of a V part
     static constexpr int VC = DP * ES / (8 * VB);                      // parts of a V row per thread
     static constexpr int VK = SB / 4;                                  // V rows per thread
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
                 // a row's address once, its parts at constant distances; rows that no one sees
                 // give zeros
                 auto rows_of = [&](auto whole) {
-                    if (!is_v) {
+                    if (!is_v && F::K_PRIVATE) {
 #pragma unroll
                         for (int n = 0; n < F::NT; n++) {
                             const uint32_t o = __shfl_sync(0xffffffffu, off, sub * F::SB + n * 8 + g);
@@ -249,6 +254,14 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
                                 const bool in = decltype(whole)::value || i * 64 + t * 16 < D * F::ES;
                                 copy_part<16>(at + ((n * F::KC + i) * 32 + lane) * 16, in ? row + i * 64 : kb, live && in);
                             }
+                        }
+                    } else if (!is_v) {   // whole rows by neighbouring lanes; odd rows' halves of 128 bytes change places
+#pragma unroll
+                        for (int i = 0; i < F::HALF / 512; i++) {
+                            const int r = i * F::K_ROWS + lane / F::K_LANES, unit = lane % F::K_LANES;
+                            const uint32_t o = __shfl_sync(0xffffffffu, off, sub * F::SB + r);
+                            const bool live = o != ~0u && (decltype(whole)::value || unit * 16 < D * F::ES);
+                            copy_part<16>(at + r * DP * F::ES + ((unit ^ (r & 1) << 2) << 4), live ? kb + ((uint64_t)o << 4) + unit * 16 : kb, live);
                         }
                     } else {
 #pragma unroll
@@ -416,7 +429,7 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             for (int i = 0; i < F::KC; i++) {
                 uint32_t kr[F::NT][4];
 #pragma unroll
-                for (int n = 0; n < F::NT; n++) read_part(kr[n], k_at + ((n * F::KC + i) * 32 + lane) * 16);
+                for (int n = 0; n < F::NT; n++) read_part(kr[n], k_at + (F::K_PRIVATE ? ((n * F::KC + i) * 32 + lane) << 4 : (n * 8 + g) * DP * F::ES + ((i ^ (g & 1)) * 4 + t << 4)));
 #pragma unroll
                 for (int e = 0; e < PER; e++) {
                     const int st = i * PER + e;
@@ -801,7 +814,8 @@ constexpr int MAX_BLOCKS_PER_SM = 3;
 // run as one launch, every item in one block: the join would cost more than it
 // spreads.  Blocks take a group of heads when there are enough items even then
 // (heads of the same positions lie next to each other, and warps have nothing
-// to add up), one head when items have to be cut into many parts.
+// to add up: 64 sequences over int8 193 -> 166 us), one head when items have to
+// be cut into many parts (2 x 65536 positions over int8: 75 -> 58 us).
 constexpr int WHOLE_KEYS = 512;
 constexpr int MIN_POSITIONS = 256;   // of a block's share
 struct Spread {
@@ -825,7 +839,7 @@ Spread few_spread(const RtPagedAttention& p, int per_sm) {
     const int64_t tiles = (int64_t)p.n_seqs * ((rows + s.rows - 1) / s.rows), positions = std::max(p.max_kv, 1);
     s.head_group = 1;
     while (!s.whole && s.head_group < FW && p.cache.n_heads % (2 * s.head_group) == 0 &&
-           tiles * (p.cache.n_heads / (2 * s.head_group)) * 6 >= g_num_sms * MAX_BLOCKS_PER_SM)
+           tiles * (p.cache.n_heads / (2 * s.head_group)) * 6 >= (int64_t)g_num_sms * (s.rows == 32 ? 2 : MAX_BLOCKS_PER_SM))
         s.head_group *= 2;
     s.key_shift = s.head_group == 1 ? 7 : s.head_group == 2 ? 6 : 5;
     const int64_t items = tiles * (p.cache.n_heads / s.head_group);

@@ -91,14 +91,17 @@ __device__ __forceinline__ int paged_row_tiles(const PagedArgs& p, const PagedSe
 }
 
 template <int R>
-__device__ __forceinline__ int paged_units(const PagedArgs& p, int b) {
-    if (b >= p.a.n_seqs) return 0;
-    const PagedSeq s = paged_seq(p, b);
+__device__ __forceinline__ int paged_units(const PagedArgs& p, const PagedSeq& s) {
     const int nq = paged_row_tiles<R>(p, s);
     if (p.whole) return nq * p.head_groups;
     int sum = 0;
     for (int q = 0; q < nq; q++) sum += paged_tiles<R>(p, s, q).count;
     return sum * p.head_groups;
+}
+
+template <int R>
+__device__ __forceinline__ int paged_units(const PagedArgs& p, int b) {
+    return b >= p.a.n_seqs ? 0 : paged_units<R>(p, paged_seq(p, b));
 }
 
 // Inclusive sum over the block's T threads; `total` gets the block's sum.
@@ -157,12 +160,51 @@ struct PagedCursor {
 template <int T, int R>
 __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, int blocks, int* sh, PagedCursor& c, int& u,
                                                int& per, int& total) {
-    int mine = paged_units<R>(p, threadIdx.x), all;
+    auto settle = [&](int r) {   // row tile, then head group and key tile, from units after the sequence's first
+        while (true) {
+            const int per_head = p.whole ? 1 : c.t.count, n = per_head * p.head_groups;
+            if (r < n) {
+                c.h = r / per_head;
+                c.i = r % per_head;
+                return;
+            }
+            r -= n;
+            c.t = paged_tiles<R>(p, c.s, ++c.qt);
+        }
+    };
+    if (p.a.n_seqs <= 32) {   // every warp for itself, a lane per sequence: no barrier, every length read once
+        const int lane = threadIdx.x & 31;
+        PagedSeq s = {lane, 0, 0, 0};
+        if (lane < p.a.n_seqs) s = paged_seq(p, lane);
+        const int mine = s.n > 0 ? paged_units<R>(p, s) : 0;
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        total = __shfl_sync(0xffffffffu, incl, 31);
+        per = max(p.min_units, (total + blocks - 1) / blocks);
+        u = (int)min((int64_t)block * per, (int64_t)0x7fffffff);
+        if (u >= total) return false;
+        const int from = __ffs(__ballot_sync(0xffffffffu, u < incl)) - 1;
+        c.s.b = from;
+        c.s.first = __shfl_sync(0xffffffffu, s.first, from);
+        c.s.n = __shfl_sync(0xffffffffu, s.n, from);
+        c.s.L = __shfl_sync(0xffffffffu, s.L, from);
+        const int r = u - __shfl_sync(0xffffffffu, incl - mine, from);
+        c.qt = c.h = c.i = 0;
+        c.nq = paged_row_tiles<R>(p, c.s);
+        c.t = paged_tiles<R>(p, c.s, 0);
+        settle(r);
+        return true;
+    }
+    int mine = paged_units<R>(p, (int)threadIdx.x), all;
     int incl = paged_scan<T>(mine, sh, &all);
     total = all;
     for (int base = T; base < p.a.n_seqs; base += T) {
         int part;
-        paged_scan<T>(paged_units<R>(p, base + threadIdx.x), sh, &part);
+        paged_scan<T>(paged_units<R>(p, base + (int)threadIdx.x), sh, &part);
         total += part;
     }
     per = max(p.min_units, (total + blocks - 1) / blocks);
@@ -171,7 +213,7 @@ __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, in
     int carry = 0;
     for (int base = 0;; base += T) {
         if (base) {
-            mine = paged_units<R>(p, base + threadIdx.x);
+            mine = paged_units<R>(p, base + (int)threadIdx.x);
             incl = paged_scan<T>(mine, sh, &all);
         }
         const int first = carry + incl - mine;
@@ -184,19 +226,11 @@ __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, in
     }
     __syncthreads();
     const int b = sh[T / 32];
-    int r = u - sh[T / 32 + 1];
+    const int r = u - sh[T / 32 + 1];
     __syncthreads();
     c.open<R>(p, b);
-    while (true) {   // row tile, then head and key tile
-        const int per_head = p.whole ? 1 : c.t.count, n = per_head * p.head_groups;
-        if (r < n) {
-            c.h = r / per_head;
-            c.i = r % per_head;
-            return true;
-        }
-        r -= n;
-        c.t = paged_tiles<R>(p, c.s, ++c.qt);
-    }
+    settle(r);
+    return true;
 }
 
 // Position -> page and slot in it.
