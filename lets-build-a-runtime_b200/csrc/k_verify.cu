@@ -13,12 +13,24 @@
 // Only the row where a sequence stops is read, once: 8 bytes per entry of the
 // vocabulary in fp32, bound by HBM for many sequences and by latency for few.
 // A cluster of up to 8 blocks takes a sequence, each a slice of the row: a
-// block settles the drafts by itself (a few loads), sums its slice while it
-// keeps the weights in shared memory, sends its sum to the others, and the one
-// in whose slice the running sum crosses finds the token there.
+// block settles the drafts by itself (a few loads), sums its slice, sends its
+// sum to the others, and the one in whose slice the running sum crosses finds
+// the token there.  A slice streams through a ring in shared memory that bulk
+// copies fill (rows of any alignment: what lies before the first and after the
+// last 16-byte boundary is loaded and stored by threads).  Sums are kept for
+// every piece, so only the piece with the token is looked at again.
+//
+// A warp copies, the others sum: what a block has under way is then bound by
+// the ring alone, and one block of 16 + 1 warps per SM with six slots of 2 x 16
+// KB does better than several smaller ones (128 rows of 131071 entries, fp32
+// target and draft, 134 MB: 24 us = 5.6 TB/s; two blocks with 5 x 16 KB 30,
+// three with 3 x 16 KB 35; loads into registers without a ring 50).  One
+// sequence of 32000 entries takes 6.5 us, of which the loads that follow from
+// one another (lengths, drafts, their probabilities, the row) are the most.
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "rt_internal.h"
 #include "sm100_ptx.h"
@@ -26,15 +38,20 @@
 namespace rt {
 namespace {
 
-constexpr int VT = 512, MAX_CLUSTER = 8;
-constexpr int STAGED = 4096;   // weights of a slice kept in shared memory; the one longer slice that holds the token is read again (L2)
+constexpr int VT = 512, MAX_CLUSTER = 8, BLOCKS_PER_SM = 1;   // VT threads that sum, and a warp that copies
+constexpr int PIECE = 16384, SLOTS = 6;          // bytes of a row in a slot; slots
+constexpr int ROW_SLOT = PIECE + 16;             // (a piece may start anywhere in its first 16 bytes)
+constexpr int GROUPS = 128;                      // sums kept per slice, each of 2^k pieces
+constexpr int RING_BYTES = SLOTS * 2 * ROW_SLOT;
+constexpr int KERR_WAIT = 0x351;
+constexpr uint64_t WAIT_NS = 200000000ull;
 
 // w = a - b, clamped to [0, 1] (NaN: 0), in units of 2^-40, truncated: the
 // steps of 2^-20 below it by adding 8 with rounding toward zero (whose last
 // place is 2^-20), then the steps of 2^-40 of what is left, which is exact.
 // Two 32-bit counts instead of a 64-bit integer: conversions to 64 bits run at
-// a fraction of the rate, and a thread's counts fit (2^20 per entry, at most
-// 2^22 / 512 entries).
+// a fraction of the rate, and the counts of a warp's entries in a group fit
+// (2^20 per entry, at most 2^11 entries).
 __device__ __forceinline__ void weight(float a, float b, uint32_t& hi, uint32_t& lo) {
     float w;
     asm("sub.sat.f32 %0, %1, %2;" : "=f"(w) : "f"(a), "f"(b));
@@ -46,91 +63,185 @@ __device__ __forceinline__ void weight(float a, float b, uint32_t& hi, uint32_t&
 __device__ __forceinline__ float load_prob(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float load_prob(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
 __device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
+__device__ __forceinline__ unsigned long long warp_scan(unsigned long long x, int lane) {   // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+// Entries [0, size) of a row from `base` (any alignment) as pieces in a ring.
+template <class T>
+struct RowPieces {
+    static constexpr int C = PIECE / (int)sizeof(T);   // entries of a piece
+    uint64_t base, end;
+    uint32_t off;   // of the first entry in its 16 bytes
+    __device__ RowPieces(const T* p, int size)
+        : base(reinterpret_cast<uint64_t>(p)), end(base + (uint64_t)size * sizeof(T)), off((uint32_t)base & 15) {}
+    // The 16-byte parts of piece c that lie within the row.
+    __device__ __forceinline__ void bounds(int c, uint64_t& from, uint32_t& bytes) const {
+        const uint64_t a = base + (uint64_t)c * PIECE, b = a + PIECE;
+        from = c ? a & ~15ull : (a + 15) & ~15ull;
+        const uint64_t to = min((b + 15) & ~15ull, end & ~15ull);
+        bytes = to > from ? (uint32_t)(to - from) : 0;
+    }
+    // Its place in the slot is that of the row, so every piece starts at `off`.
+    __device__ __forceinline__ uint32_t copy(int c, uint8_t* slot, uint64_t* bar) const {
+        uint64_t from;
+        uint32_t bytes;
+        bounds(c, from, bytes);
+        if (bytes) ptx::bulk_load(slot + (uint32_t)(from - (base - off + (uint64_t)c * PIECE)), reinterpret_cast<const void*>(from), bytes, bar);
+        return bytes;
+    }
+    // The rest of piece c, an entry for each of 32 / sizeof(T) lanes: what lies before the copied
+    // part and after it (less than 16 bytes each), or all of the piece if that is less than 32.
+    __device__ __forceinline__ void edges(int c, uint8_t* slot, int e) const {
+        constexpr int HALF = 16 / (int)sizeof(T);
+        uint64_t from;
+        uint32_t bytes;
+        bounds(c, from, bytes);
+        const uint64_t first = base + (uint64_t)c * PIECE, last = min(end, first + PIECE);
+        const bool after = bytes && e >= HALF;
+        const uint64_t at = after ? from + bytes + (e - HALF) * sizeof(T) : first + e * sizeof(T);
+        if (at >= (after || !bytes ? last : from)) return;
+        *reinterpret_cast<T*>(slot + (uint32_t)(at - (base - off + (uint64_t)c * PIECE))) = *reinterpret_cast<const T*>(at);
+        ptx::fence_proxy_async_smem();   // a later piece's copy writes here
+    }
+};
 
 template <class T>
-__global__ void __launch_bounds__(VT, 3) verify_kernel(RtVerifyDraft v, int blocks, int slice, int* err) {
-    extern __shared__ float kept[];                       // weights of the slice, before fixed point
-    __shared__ unsigned long long sums[VT / 32], share[2][MAX_CLUSTER];
-    __shared__ int first;
+__global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __grid_constant__ RtVerifyDraft v, int blocks, int slice, int group_shift, int* err) {
+    constexpr int C = RowPieces<T>::C, PER = C / VT;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ unsigned long long parts[GROUPS][VT / 32], group_sums[GROUPS], sums[VT / 32], share[2][MAX_CLUSTER];
+    __shared__ uint64_t full[SLOTS], empty[SLOTS];
+    __shared__ int first, abort_flag;
     const int b = blockIdx.y, rank = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const int N = v.n_drafts, V = v.vocab;
     const T* target = static_cast<const T*>(v.target) + b * v.target_stride[0];
     const T* draft = v.draft ? static_cast<const T*>(v.draft) + b * v.draft_stride[0] : nullptr;
 
     // ---- how many drafts stand ----
+    if (t == 0) {
+        first = N;
+        abort_flag = 0;
+        for (int i = 0; i < SLOTS; i++) {
+            ptx::mbar_init(&full[i], 1);
+            ptx::mbar_init(&empty[i], VT / 32);
+        }
+        ptx::fence_mbar_init();
+    }
     int limit = v.draft_lens ? v.draft_lens[b] : N;
+    const float u = v.sample_u[b];
+    __syncthreads();
+    for (int i = t; i < N; i += VT + 32) {   // (what lies beyond the limit is loaded along with it and not looked at)
+        const int x = v.draft_tokens[b * N + i];
+        const float au = v.accept_u[b * N + i];
+        const bool known = x >= 0 && x < V;
+        float p = 0.0f, q = 1.0f;
+        if (known) {
+            p = load_prob(target + i * v.target_stride[1] + x);
+            if (draft) q = load_prob(draft + i * v.draft_stride[1] + x);
+        }
+        if (i < limit) {
+            if (!known && rank == 0) atomicCAS(err, 0, KERR_TOKEN);
+            if (!known || !(__fmul_rn(au, q) < p)) atomicMin(&first, i);
+        }
+    }
     if (limit < 0 || limit > N) {
         if (t == 0) atomicCAS(err, 0, KERR_LENGTH);
         limit = limit < 0 ? 0 : N;
     }
-    if (t == 0) first = limit;
     __syncthreads();
-    for (int i = t; i < limit; i += VT) {
-        const int x = v.draft_tokens[b * N + i];
-        const float u = v.accept_u[b * N + i];
-        bool keep = false;
-        if (x < 0 || x >= V) {
-            if (rank == 0) atomicCAS(err, 0, KERR_TOKEN);
-        } else {
-            const float p = load_prob(target + i * v.target_stride[1] + x);
-            const float q = draft ? load_prob(draft + i * v.draft_stride[1] + x) : 1.0f;
-            keep = __fmul_rn(u, q) < p;
-        }
-        if (!keep) atomicMin(&first, i);
-    }
-    __syncthreads();
-    const int n = first;
-    const T* row = target + n * v.target_stride[1];
+    const int n = min(first, limit);
     bool residual = n < limit;
+    const T* row = target + n * v.target_stride[1];
     const T* qrow = draft && residual ? draft + n * v.draft_stride[1] : nullptr;
     const int point = !draft && residual ? v.draft_tokens[b * N + n] : -1;   // a certain draft: q is 1 there
-    const int lo = min(V, rank * slice), size = min(V, lo + slice) - lo;
-    const bool keep_all = slice <= STAGED;
-    const float u = v.sample_u[b];
+    const int lo = min(V, rank * slice), size = min(V, lo + slice) - lo, pieces = (size + C - 1) / C;
     row += lo;
     if (qrow) qrow += lo;
-    // What is taken off the target at entry i of the slice.
-    auto taken = [&](int i) -> float {
-        if (!residual) return 0.0f;
-        return qrow ? load_prob(qrow + i) : (lo + i == point ? 1.0f : 0.0f);
-    };
+    const RowPieces<T> ps(row, size), qs(qrow ? qrow : row, size);
 
     // ---- the slice's sum, and everybody's ----
     unsigned long long total = 0;
+    const int group_mask = (1 << group_shift) - 1;
+    int slot = 0, phase = 0, slot0 = 0;   // slot0: the pass's first
     for (int pass = 0; pass < 2; pass++) {
-        uint32_t hi = 0, lo20 = 0;
-        for (int i0 = t; i0 < size; i0 += 8 * VT) {
-            float p[8], q[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) p[k] = i0 + k * VT < size ? load_prob(row + i0 + k * VT) : 0.0f;
-            if (residual && qrow) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) q[k] = i0 + k * VT < size ? load_prob(qrow + i0 + k * VT) : 0.0f;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; k++) q[k] = taken(i0 + k * VT);
+        const bool two = residual && qrow;
+        slot0 = slot;
+        if (warp == VT / 32) {
+            for (int c = 0; c < pieces; c++) {
+                uint8_t* at = ring + slot * 2 * ROW_SLOT;
+                // (a slot's n-th filling waits for its (n - 1)-th emptying; the first for none)
+                ptx::wait_short(&empty[slot], phase ^ 1, &abort_flag, err, KERR_WAIT, WAIT_NS);
+                uint32_t bytes = 0;
+                if (lane == 0) {
+                    bytes = ps.copy(c, at, &full[slot]);
+                    if (two) bytes += qs.copy(c, at + ROW_SLOT, &full[slot]);
+                }
+                if (c == 0 || c >= pieces - 2) {
+                    if (lane < 32 / sizeof(T)) ps.edges(c, at, lane);
+                    if (two && lane < 32 / sizeof(T)) qs.edges(c, at + ROW_SLOT, lane);
+                    __syncwarp();
+                }
+                if (lane == 0) ptx::mbar_expect_tx(&full[slot], bytes);
+                if (++slot == SLOTS) slot = 0, phase ^= 1;
             }
+        } else {
+            uint32_t hi = 0, lo20 = 0;
+            for (int c = 0; c < pieces; c++) {
+                ptx::wait_short(&full[slot], phase, &abort_flag, err, KERR_WAIT, WAIT_NS);
+                const T* p = reinterpret_cast<const T*>(ring + slot * 2 * ROW_SLOT + ps.off) + t;
+                const T* q = reinterpret_cast<const T*>(ring + slot * 2 * ROW_SLOT + ROW_SLOT + qs.off) + t;
+                auto sum = [&](auto whole, auto with_q) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                uint32_t h, l;
-                weight(p[k], q[k], h, l);
-                hi += h;
-                lo20 += l;
-                if (keep_all && i0 + k * VT < size) kept[i0 + k * VT] = p[k] - q[k];
+                    for (int k = 0; k < PER; k++) {
+                        const int i = c * C + k * VT + t;
+                        uint32_t h = 0, l = 0;
+                        if (decltype(whole)::value || i < size)
+                            weight(to_float(p[k * VT]), decltype(with_q)::value ? to_float(q[k * VT]) : lo + i == point ? 1.0f : 0.0f, h, l);
+                        hi += h;
+                        lo20 += l;
+                    }
+                };
+                const bool whole = (c + 1) * C <= size;
+                if (two) whole ? sum(std::true_type(), std::true_type()) : sum(std::false_type(), std::true_type());
+                else whole ? sum(std::true_type(), std::false_type()) : sum(std::false_type(), std::false_type());
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&empty[slot]);
+                if (++slot == SLOTS) slot = 0, phase ^= 1;
+                if ((c & group_mask) == group_mask || c == pieces - 1) {
+                    hi = __reduce_add_sync(0xffffffffu, hi);
+                    lo20 = __reduce_add_sync(0xffffffffu, lo20);
+                    if (lane == 0) parts[c >> group_shift][warp] = ((unsigned long long)hi << 20) + lo20;
+                    hi = lo20 = 0;
+                }
             }
         }
-        unsigned long long mine = ((unsigned long long)hi << 20) + lo20;
-        mine = warp_sum(mine);
+        const int groups = (pieces + group_mask) >> group_shift;
         __syncthreads();
-        if (lane == 0) sums[warp] = mine;
+        if (t < groups) {
+            unsigned long long x = 0;
+#pragma unroll
+            for (int k = 0; k < VT / 32; k++) x += parts[t][(k + t) % (VT / 32)];
+            group_sums[t] = x;
+        }
         __syncthreads();
         if (warp == 0) {
-            mine = warp_sum(lane < VT / 32 ? sums[lane] : 0ull);
+            unsigned long long mine = 0;
+            for (int i = lane; i < groups; i += 32) mine += group_sums[i];
+            mine = warp_sum(mine);
             if (lane < blocks) {   // to the same place in every block of the cluster
                 const uint32_t dst = ptx::mapa_shared(ptx::smem_u32(&share[pass][rank]), lane);
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst), "l"(mine) : "memory");
@@ -147,32 +258,86 @@ __global__ void __launch_bounds__(VT, 3) verify_kernel(RtVerifyDraft v, int bloc
             const unsigned long long cut = m * (total >> 24) + ((m * (total & 0xffffffull)) >> 24);
             // ---- the token, in the slice where the sum crosses ----
             if (total && before <= cut && cut < before + share[pass][rank]) {
-                // a warp takes consecutive entries, a lane every 32nd of them; then one warp's
-                // entries again, in order
-                const int per = ((size + VT / 32 - 1) / (VT / 32) + 31) & ~31, w0 = min(size, warp * per), w1 = min(size, w0 + per);
-                auto again = [&](int i) -> unsigned long long {
-                    uint32_t h, l;
-                    if (keep_all) weight(kept[i], 0.0f, h, l);
-                    else weight(load_prob(row + i), taken(i), h, l);
-                    return ((unsigned long long)h << 20) + l;
+                // the group of pieces (every warp finds it for itself) ...
+                int group = 0;
+                for (int i = 0; i < groups; i += 32) {
+                    unsigned long long x = i + lane < groups ? group_sums[i + lane] : 0ull;
+                    const unsigned long long own = x;
+                    x = warp_scan(x, lane);
+                    const uint32_t over = __ballot_sync(0xffffffffu, before + x > cut);
+                    if (over) {
+                        const int at = __ffs(over) - 1;
+                        group = i + at;
+                        before += __shfl_sync(0xffffffffu, x - own, at);
+                        break;
+                    }
+                    before += __shfl_sync(0xffffffffu, x, 31);
+                }
+                // ... a lane takes EACH consecutive entries of it, a warp 32 times that (often
+                // enough for longer groups); then the lane's entries in order
+                constexpr int EACH = PER;
+                const int g_from = group * C << group_shift, g_to = min(size, g_from + (C << group_shift));
+                const bool in_ring = pieces <= SLOTS;
+                float p[EACH], q[EACH];
+                auto load = [&](int from) {   // this lane's entries, zeros past the end
+#pragma unroll
+                    for (int k = 0; k < EACH; k++) {
+                        const int i = from + k;
+                        p[k] = 0.0f;
+                        q[k] = lo + i == point && residual ? 1.0f : 0.0f;
+                        if (i >= g_to) continue;
+                        if (in_ring) {
+                            const uint8_t* at = ring + (slot0 + i / C) % SLOTS * 2 * ROW_SLOT;
+                            p[k] = to_float(reinterpret_cast<const T*>(at + ps.off)[i % C]);
+                            if (two) q[k] = to_float(reinterpret_cast<const T*>(at + ROW_SLOT + qs.off)[i % C]);
+                        } else {   // (from L2)
+                            p[k] = load_prob(row + i);
+                            if (two) q[k] = load_prob(qrow + i);
+                        }
+                    }
                 };
-                unsigned long long part = 0;
-                for (int i = w0 + lane; i < w1; i += 32) part += again(i);
-                part = warp_sum(part);
-                if (lane == 0) sums[warp] = part;
+                auto sum = [&] {
+                    uint32_t hi = 0, lo20 = 0, h, l;
+#pragma unroll
+                    for (int k = 0; k < EACH; k++) {
+                        weight(p[k], q[k], h, l);
+                        hi += h;
+                        lo20 += l;
+                    }
+                    return ((unsigned long long)hi << 20) + lo20;
+                };
+                const int steps = 1 << group_shift, w_from = g_from + warp * 32 * EACH * steps + lane * EACH;
+                unsigned long long part = 0, x = 0;
+                if (warp < VT / 32) {
+                    for (int i = 0; i < steps; i++) {
+                        load(w_from + i * 32 * EACH);
+                        x = warp_scan(sum(), lane);
+                        part += __shfl_sync(0xffffffffu, x, 31);
+                    }
+                    if (lane == 0) sums[warp] = part;
+                }
                 __syncthreads();
                 for (int k = 0; k < warp; k++) before += sums[k];
                 if (before <= cut && cut < before + part) {
-                    for (int i = w0; i < w1; i += 32) {
-                        unsigned long long x = i + lane < w1 ? again(i + lane) : 0ull;
-#pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-                            if (lane >= o) x += y;
+                    for (int i = 0; i < steps; i++) {
+                        if (steps > 1) {
+                            load(w_from + i * 32 * EACH);
+                            x = warp_scan(sum(), lane);
                         }
                         const uint32_t over = __ballot_sync(0xffffffffu, before + x > cut);
                         if (over) {
-                            if (lane == 0) v.tokens[b * (N + 1) + n] = lo + i + __ffs(over) - 1;
+                            before += __shfl_up_sync(0xffffffffu, x, 1) * (lane > 0);
+                            if (lane == __ffs(over) - 1) {
+                                int token = w_from + i * 32 * EACH;
+#pragma unroll
+                                for (int k = 0; k < EACH - 1; k++) {
+                                    uint32_t h, l;
+                                    weight(p[k], q[k], h, l);
+                                    before += ((unsigned long long)h << 20) + l;
+                                    token += before <= cut;
+                                }
+                                v.tokens[b * (N + 1) + n] = lo + token;
+                            }
                             break;
                         }
                         before += __shfl_sync(0xffffffffu, x, 31);
@@ -184,7 +349,7 @@ __global__ void __launch_bounds__(VT, 3) verify_kernel(RtVerifyDraft v, int bloc
         residual = false;   // nothing left of the residual: the target's own row
     }
     if (rank == 0) {
-        for (int i = t; i <= N; i += VT)
+        for (int i = t; i <= N; i += VT + 32)
             if (i != n || !total) v.tokens[b * (N + 1) + i] = i < n ? v.draft_tokens[b * N + i] : -1;
         if (t == 0) v.accepted[b] = n;
     }
@@ -192,15 +357,19 @@ __global__ void __launch_bounds__(VT, 3) verify_kernel(RtVerifyDraft v, int bloc
 
 template <class T>
 Status verify_as(const RtVerifyDraft& v, cudaStream_t st) {
-    static const cudaError_t set = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, STAGED * 4);
+    static const cudaError_t set = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES);
     RT_CUDA_CHECK(set);
-    int blocks = MAX_CLUSTER;
-    while (blocks > 1 && v.vocab < blocks * 1024) blocks /= 2;   // a slice of less than two loads a thread is not worth a block
+    // as many blocks a sequence as are resident at once, of two loads a thread at least
+    int blocks = std::max(1, std::min(MAX_CLUSTER, BLOCKS_PER_SM * g_num_sms / v.n_seqs));
+    while (blocks > 1 && v.vocab < blocks * 1024) blocks--;
     const int slice = (v.vocab + blocks - 1) / blocks;
+    int group_shift = 0;
+    while (((slice + RowPieces<T>::C - 1) / RowPieces<T>::C) > GROUPS << group_shift) group_shift++;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, v.n_seqs);
-    cfg.blockDim = dim3(VT);
-    cfg.dynamicSmemBytes = slice <= STAGED ? slice * 4 : 0;
+    cfg.blockDim = dim3(VT + 32);
+    // (a call's two passes over a short slice use a slot a piece each)
+    cfg.dynamicSmemBytes = std::min(SLOTS, 2 * ((slice + RowPieces<T>::C - 1) / RowPieces<T>::C)) * 2 * ROW_SLOT;
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -208,7 +377,7 @@ Status verify_as(const RtVerifyDraft& v, cudaStream_t st) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T>, v, blocks, slice, kernel_error_flag()));
+    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T>, v, blocks, slice, group_shift, kernel_error_flag()));
     return Status::ok();
 }
 

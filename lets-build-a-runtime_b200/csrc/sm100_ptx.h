@@ -64,6 +64,15 @@ __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, vol
     }
 }
 
+// The same for waits that are short as a rule: the clock is read only after
+// some tries in vain (a try sleeps by itself for a while).
+__device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                           int* err, int code, uint64_t limit_ns) {
+    for (int i = 0; i < 16; i++)
+        if (mbar_try_wait(bar, parity)) return true;
+    return wait_bounded(bar, parity, abort_flag, err, code, limit_ns);
+}
+
 // 3-D tiled TMA load into shared memory, completion counted on `bar`.
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int c0, int c1,
                                             int c2) {
