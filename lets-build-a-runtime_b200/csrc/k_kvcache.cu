@@ -21,27 +21,25 @@ template <class A> struct Unit;   // one lane's features of the dense side
 template <> struct Unit<float> { static constexpr int N = 4; };
 template <> struct Unit<__nv_bfloat16> { static constexpr int N = 8; };
 
-__device__ __forceinline__ void load_unit(const float* p, bool vec, float (&x)[4]) {
-    if (vec) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = p[i];
-    }
+// Both are 16 bytes: loaded as they are, and given their values later.
+__device__ __forceinline__ uint4 load_unit(const float* p, bool vec) {
+    if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+    return make_uint4(__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3]));
 }
-__device__ __forceinline__ void load_unit(const __nv_bfloat16* p, bool vec, float (&x)[8]) {
-    if (vec) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ uint4 load_unit(const __nv_bfloat16* p, bool vec) {
+    if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+}
+__device__ __forceinline__ void unit_values(uint4 v, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unit_values(uint4 v, float (&x)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __bfloat162float(p[i]);
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
 __device__ __forceinline__ uint32_t bf16_two(float a, float b) {   // a in the low half
@@ -86,9 +84,11 @@ __device__ __forceinline__ void put_cache(void* base, int64_t off, const float (
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
             if constexpr (CT == RT_I8) {
-                w[i] = 0;
+                // to the nearest, ties to even, by adding 1.5 * 2^23: the low byte is the code (|x| <= 128)
+                uint32_t b[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) w[i] |= ((uint32_t)__float2int_rn(x[4 * i + j]) & 0xffu) << (8 * j);
+                for (int j = 0; j < 4; j++) b[j] = __float_as_uint(__fadd_rn(x[4 * i + j], 12582912.0f));
+                w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
             } else {   // satfinite, to the nearest, ties to even
                 const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
                 const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
@@ -176,64 +176,86 @@ __device__ __forceinline__ Place place_of(const RtKvCache& c, int64_t page, int 
     return {page * c.stride[0] + off * c.stride[1], page * c.scale_stride[0] + off * c.scale_stride[1]};
 }
 
-// A thread has its part of WRITE_BATCH tokens under way at a time.
-constexpr int WRITE_BATCH = 4;
+// The largest |x| of a unit, as bits: NaN and infinity come out on top.
+__device__ __forceinline__ uint32_t unit_top(uint4 v, float) {
+    return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+}
+__device__ __forceinline__ uint32_t unit_top(uint4 v, __nv_bfloat16) {
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+}
+
+// A lane of every warp looks one of the block's tokens up, and hands its place
+// to the others as they come to it (no barrier; a look-up by every thread for
+// itself cost as much as the rest of its work).  A thread loads its part of
+// WRITE_BATCH tokens while it works on those before.
+constexpr int WRITE_TOKENS = 8, WRITE_BATCH = 2;
 template <class A, int CT>
 __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const __grid_constant__ RtKvWrite w, const __grid_constant__ RowMap m, bool vec, int* err) {
     constexpr int N = Unit<A>::N;
+    constexpr bool SCALED = CT == RT_I8 || CT == RT_F8E4M3;
     const RtKvCache& c = w.cache;
     const Part x = part_of(m, c.n_heads);
     const int64_t* st = x.is_v ? w.v_stride : w.k_stride;
-    const A* src = static_cast<const A*>(x.is_v ? w.v : w.k) + x.head * st[1] + x.unit * N;
+    const int t0 = blockIdx.x * m.tokens, n = min(m.tokens, w.n_tokens - t0);
+    const A* src = static_cast<const A*>(x.is_v ? w.v : w.k) + (t0 + (int)threadIdx.y) * st[0] + x.head * st[1] + x.unit * N;
+    const int64_t step = blockDim.y * st[0];
     void* dst = x.is_v ? c.v : c.k;
     float* scales = x.is_v ? c.v_scale : c.k_scale;
     const int64_t at = x.head * c.stride[2] + x.unit * N, scale_at = x.head * c.scale_stride[2];
-    const int t0 = blockIdx.x * m.tokens, n = min(m.tokens, w.n_tokens - t0);
-    for (int b0 = 0; b0 < n; b0 += WRITE_BATCH * blockDim.y) {   // (all lanes of a warp alike, for the shuffles)
-        const int b = b0 + threadIdx.y;
-        float v[WRITE_BATCH][N];
-        int64_t slots[WRITE_BATCH];
+    const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31;
+    const int64_t slot = lane < n ? w.slots[t0 + lane] : -1;
+    uint4 next[WRITE_BATCH];
+    auto load = [&](int b) {
 #pragma unroll
         for (int i = 0; i < WRITE_BATCH; i++) {
-            const int token = b + i * blockDim.y;
-            slots[i] = token < n ? w.slots[t0 + token] : -1;
-            if (token < n && x.live) {
-                load_unit(src + (t0 + token) * st[0], vec, v[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; j++) v[i][j] = 0.0f;
-            }
+            next[i] = make_uint4(0, 0, 0, 0);
+            if (x.live && b + i * (int)blockDim.y < n) next[i] = load_unit(src, vec);
+            src += step;
         }
+    };
+    load(threadIdx.y);
+    Place mine = {-1, 0};
+    if (slot >= (int64_t)c.n_pages * c.page_size) {
+        atomicCAS(err, 0, KERR_SLOT);
+    } else if (slot >= 0) {
+        const uint32_t page = ((uint32_t)slot + __umulhi((uint32_t)slot, m.page_mul)) >> m.page_shift;
+        mine = place_of(c, page, (int)((uint32_t)slot - page * c.page_size));
+    }
+    for (int b0 = 0; b0 < n; b0 += WRITE_BATCH * blockDim.y) {   // (all lanes of a warp alike, for the shuffles)
+        uint4 now[WRITE_BATCH];
+#pragma unroll
+        for (int i = 0; i < WRITE_BATCH; i++) now[i] = next[i];
+        load(b0 + threadIdx.y + WRITE_BATCH * blockDim.y);
 #pragma unroll
         for (int i = 0; i < WRITE_BATCH; i++) {
-            float scale = 0.0f;
-            if constexpr (CT == RT_I8 || CT == RT_F8E4M3) {
+            const int token = b0 + threadIdx.y + i * blockDim.y;   // (a lane past the last holds "nowhere")
+            Place p = {__shfl_sync(0xffffffffu, mine.at, token), 0};
+            if constexpr (SCALED) p.scale = __shfl_sync(0xffffffffu, mine.scale, token);
+            if (token >= n) p.at = -1;
+            float v[N], scale = 0.0f, inv = 1.0f;
+            if constexpr (SCALED) {
                 constexpr float MAX_CODE = CT == RT_I8 ? 127.0f : 448.0f;
-                // the maximum over the bits of |x|: NaN and infinity come out on top
-                uint32_t top = 0;
-#pragma unroll
-                for (int j = 0; j < N; j++) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+                uint32_t top = unit_top(now[i], A());
                 for (int o = 1 << m.lanes_log2 >> 1; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const float a = __uint_as_float(top);
                 // scale = a (1/M) and code = round(x ((1/a) M)), each step rounded to fp32:
                 // a function of the row that any fp32 arithmetic reproduces bit for bit
-                float inv = __fmul_rn(__frcp_rn(a), MAX_CODE);
+                inv = __fmul_rn(__frcp_rn(a), MAX_CODE);
                 scale = __fmul_rn(a, 1.0f / MAX_CODE);
                 if (a < 7.888609052210118e-31f) scale = inv = 0.0f;                   // 2^-100: M / a overflows further down
                 if (top >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); inv = 0.0f; }
+                if (inv == 0.0f) now[i] = make_uint4(0, 0, 0, 0);
+            }
+            unit_values(now[i], v);
+            if constexpr (SCALED) {
 #pragma unroll
-                for (int j = 0; j < N; j++) v[i][j] = inv == 0.0f ? 0.0f : __fmul_rn(v[i][j], inv);
+                for (int j = 0; j < N; j++) v[j] = __fmul_rn(v[j], inv);
             }
-            if (slots[i] < 0 || !x.live) continue;
-            if (slots[i] >= (int64_t)c.n_pages * c.page_size) {
-                atomicCAS(err, 0, KERR_SLOT);
-                continue;
-            }
-            const uint32_t slot = (uint32_t)slots[i], page = (slot + __umulhi(slot, m.page_mul)) >> m.page_shift;
-            const Place p = place_of(c, page, slot - page * c.page_size);
-            if constexpr (CT == RT_I8 || CT == RT_F8E4M3)
+            if (p.at < 0 || !x.live) continue;
+            if constexpr (SCALED)
                 if (x.unit == 0) scales[p.scale + scale_at] = scale;
-            put_cache<N, CT>(dst, p.at + at, v[i]);
+            put_cache<N, CT>(dst, p.at + at, v);
         }
     }
 }
@@ -344,7 +366,7 @@ bool vector_rows(const void* p, const int64_t st[2], int dtype) {
 template <class A, int CT>
 Status write_as(const RtKvWrite& w, cudaStream_t st) {
     dim3 grid, block;
-    const RowMap m = row_map<A>(w.cache, w.n_tokens, 16, grid, block);
+    const RowMap m = row_map<A>(w.cache, w.n_tokens, WRITE_TOKENS, grid, block);
     const bool vec = vector_rows(w.k, w.k_stride, w.dtype) && vector_rows(w.v, w.v_stride, w.dtype);
     if (grid.y > 65535) return Status::err(RT_ERR_UNSUPPORTED, "kv_write: too many heads");
     kv_write_kernel<A, CT><<<grid, block, 0, st>>>(w, m, vec, kernel_error_flag());

@@ -567,3 +567,89 @@ def test_refusals(paged):
     a.k, a.dtype = k.data_ptr(), 2
     assert lib.rt_kv_write(a, None) == 7            # RT_ERR_UNSUPPORTED
     paged.check_stream()
+
+
+@pytest.mark.parametrize("cache,act", CACHES)
+@pytest.mark.parametrize("hq,hkv,dim,new", [(8, 2, 128, 5), (4, 4, 64, 33), (8, 2, 128, 9), (16, 8, 64, 16), (2, 2, 128, 31)])
+def test_attention_around_the_kernels_row_limits(paged, cache, act, hq, hkv, dim, new):
+    """16 to 36 rows a cache head, where calls change kernels."""
+    s = Setup(cache, act, hq, hkv, dim, 24, [new, 700, 2 * new + 1, 64], [new, new, new - 1, 1], seed=new)
+    compare(s, s.attend(paged), act)
+
+
+@pytest.mark.parametrize("cache,act", [("f32", "f32"), ("bf16", "bf16"), ("i8", "f32")])
+@pytest.mark.parametrize("seqs,new", [(32, 1), (33, 1), (129, 3), (600, 1), (600, 2), (40, 50)])
+def test_attention_of_many_sequences(paged, cache, act, seqs, new):
+    lens = [(37 * i) % 150 for i in range(seqs)]
+    s = Setup(cache, act, 4, 2, 64, 8, lens, [min(new, n) for n in lens], seed=seqs)
+    compare(s, s.attend(paged), act)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_offsets_beyond_32_bits(paged, new):
+    """The same sequences on pages at both ends of a cache of more than 2^32 bytes and elements a side."""
+    page, heads, dim, n_pages = 64, 8, 128, 70000
+    assert n_pages * page * heads * dim > 2 ** 32
+    big = {x: torch.empty(n_pages, page, heads, dim, dtype=torch.int8, device="cuda") for x in "kv"}
+    scale = {x: torch.empty(n_pages, page, heads, device="cuda") for x in "kv"}
+    s = Setup("i8", "f32", 16, heads, dim, page, [300, 1000], [new, new])
+    used = s.pages["k"].shape[0]
+    move = torch.arange(used, device="cuda")
+    move[1::2] = n_pages - move[1::2]
+    for x in "kv":
+        big[x][move], scale[x][move] = s.pages[x], s.scale[x]
+    table = move[s.table.long()].to(torch.int32)
+    near = s.attend(paged)
+    far = paged.paged_attention(s.q, big["k"], big["v"], table, s.lens_t, s.cu, k_scale=scale["k"], v_scale=scale["v"])
+    assert torch.equal(near, far)
+    slots = torch.tensor([n_pages * page - 1, 3 * page + 1], device="cuda")
+    k, v = (torch.randn(2, heads, dim, device="cuda") for _ in "kv")
+    paged.kv_write(k, v, big["k"], big["v"], slots, k_scale=scale["k"], v_scale=scale["v"])
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    last = torch.tensor([[n_pages - 1]], dtype=torch.int32, device="cuda")
+    start = torch.tensor([page - 1], dtype=torch.int32, device="cuda")
+    got = paged.kv_read(big["k"], big["v"], last, start, cu, 1, k_scale=scale["k"], v_scale=scale["v"])
+    for x, y in zip((k, v), got):
+        # half a code of scale, and the products' roundings
+        assert ((x[0] - y[0]).abs() <= x[0].abs().amax(-1, keepdim=True) / 127 * (0.5 + 2.0 ** -14)).all()
+    paged.check_stream()
+
+
+def settle_row(row, u):
+    """The token for each u from one row's weights, whole numbers up to 2^63."""
+    m = np.floor(np.clip(row.astype(np.float64), 0, 1) * 2.0 ** 40).astype(np.int64)
+    c = np.cumsum(m)
+    return [int(np.searchsorted(c, (int(np.floor(float(x) * 2.0 ** 24)) * int(c[-1])) >> 24, side="right")) for x in u]
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("B,V,off", [(160, 1200001, 3), (80, 40000, 5), (1, 4194304, 1), (40, 16384, 7), (3, 6, 2), (160, 21, 1)])
+def test_verify_long_rows_at_any_alignment(paged, act, B, V, off):
+    g = gen(14)
+    logits = torch.randn(V + 8, generator=g, device="cuda")
+    row = torch.softmax(3 * logits, 0).to(ACT[act])[off:off + V]
+    u = torch.rand(B, generator=g, device="cuda")
+    none = torch.zeros(B, 0, device="cuda")
+    got, acc = paged.verify_draft(row.expand(B, 1, V), None, none.to(torch.int32), none, u)
+    assert (acc == 0).all() and got[:, 0].tolist() == settle_row(row.float().cpu().numpy(), u.cpu().numpy())
+    # a refused draft whose distribution is the target's own, at another alignment: nothing is left of the
+    # difference, and the target's row is read in a second pass
+    other = torch.empty(V + 16, dtype=ACT[act], device="cuda")[off + 5:off + 5 + V].copy_(row)
+    x = torch.zeros(B, 1, dtype=torch.int32, device="cuda")
+    got, acc = paged.verify_draft(row.expand(B, 2, V), other.expand(B, 1, V), x, torch.ones(B, 1, device="cuda"), u)
+    assert (acc == 0).all() and got[:, 0].tolist() == settle_row(row.float().cpu().numpy(), u.cpu().numpy())
+    paged.check_stream()
+
+
+@pytest.mark.parametrize("heads,dim,page,lens,start", [(1, 16, 5, [1, 0, 70, 3], None), (3, 16, 7, [40] * 50, 3),
+                                                       (40, 128, 16, [5, 33], 2), (5, 80, 1, [129, 1, 2], 1)])
+@pytest.mark.parametrize("cache,act", [("f32", "bf16"), ("bf16", "f32"), ("i8", "f32"), ("f8", "bf16")])
+def test_read_shapes(paged, cache, act, heads, dim, page, lens, start):
+    s = Setup(cache, act, heads, heads, dim, page, [n + (start or 0) for n in lens], lens)
+    at = None if start is None else torch.full((len(lens),), start, dtype=torch.int32, device="cuda")
+    got = paged.kv_read(s.pages["k"], s.pages["v"], s.table, at, s.cu, sum(lens), dtype=ACT[act], **s.kw())
+    for x, y in zip("kv", got):
+        pages = s.pages[x].float() if s.scale[x] is None else s.pages[x].float() * s.scale[x][..., None]
+        want = torch.cat([pages[s.table[b].long()].flatten(0, 1)[start or 0:][:n] for b, n in enumerate(lens)])
+        assert torch.equal(y, want.to(ACT[act]))
+    paged.check_stream()
