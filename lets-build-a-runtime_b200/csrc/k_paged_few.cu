@@ -66,6 +66,10 @@ struct Few {
     static constexpr int NR = PACK ? 1 : 2 * RT;                       // rows of a thread
     static constexpr int NQ = PACK ? 1 : (F32ACT ? 2 : 1);             // instructions per query fragment
     static constexpr int NP = PACK ? 1 : (MODE == M_F16 && !F32ACT ? 1 : 2);
+    // The tensor core's sum truncates (toward zero, in steps of 2^-24 of it): over a few thousand
+    // positions of an fp32 cache the output fell short by 1.2e-6 of its value.  With fp32 outputs
+    // products are summed from zero every 8 positions, and added up in fp32 registers.
+    static constexpr bool FOLD = MODE == M_TF32 && F32ACT;
     static constexpr int KSTEP = MODE == M_TF32 ? 8 : 16;              // features per instruction
     static constexpr int KS = DP / KSTEP;
     static constexpr int SB = 32 / ES;                                 // positions per piece: 32, 16, 8
@@ -417,13 +421,13 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             const bool mixed = pos < all_lo || pos + F::SB > all_hi;           // rows see different positions of the piece
             const bool masked = mixed || (ok & ALL) != ALL;
             // ---- scores ----
-            float sc[RT][F::NT][4];
+            float sc[RT][F::NT][4], sc_lo[RT][F::NT][4];   // sc_lo: tf32, products with a lower part
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                 for (int n = 0; n < F::NT; n++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) sc[rt][n][j] = 0.0f;
+                    for (int j = 0; j < 4; j++) sc[rt][n][j] = sc_lo[rt][n][j] = 0.0f;
             constexpr int PER = F::KS / F::KC;          // steps per 16-byte part
 #pragma unroll
             for (int i = 0; i < F::KC; i++) {
@@ -472,15 +476,25 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
                         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                             for (int k = 0; k < F::NQ; k++) {
+                                float(&to)[4] = MODE == M_TF32 && k > 0 ? sc_lo[rt][n] : sc[rt][n];
                                 if constexpr (CT == RT_F32) {
-                                    mma<MODE>(sc[rt][n], a[rt][k], tf32_hi(b0), tf32_hi(b1));
-                                    mma<MODE>(sc[rt][n], a[rt][k], tf32_lo(b0), tf32_lo(b1));
+                                    mma<MODE>(to, a[rt][k], tf32_hi(b0), tf32_hi(b1));
+                                    mma<MODE>(sc_lo[rt][n], a[rt][k], tf32_lo(b0), tf32_lo(b1));
                                 } else {
-                                    mma<MODE>(sc[rt][n], a[rt][k], b0, b1);
+                                    mma<MODE>(to, a[rt][k], b0, b1);
                                 }
                             }
                     }
                 }
+            }
+
+            if constexpr (MODE == M_TF32) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int n = 0; n < F::NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) sc[rt][n][j] += sc_lo[rt][n][j];
             }
 
             // ---- weights ----
@@ -701,17 +715,23 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
                                 }
                             }
 #pragma unroll
-                            for (int rt = 0; rt < RT; rt++)
+                            for (int rt = 0; rt < RT; rt++) {
+                                float(&to)[4] = o[rt][i * F::VE + e];
+                                float acc[4];
 #pragma unroll
-                                for (int k = 0; k < F::NP; k++) {
-                                    float(&acc)[4] = o[rt][i * F::VE + e];
+                                for (int j = 0; j < 4; j++) acc[j] = F::FOLD ? 0.0f : to[j];
+#pragma unroll
+                                for (int k = F::NP - 1; k >= 0; k--) {   // the small products first: they are truncated to their own size
                                     if constexpr (CT == RT_F32) {
-                                        mma<MODE>(acc, a[rt][k], tf32_hi(b0), tf32_hi(b1));
                                         mma<MODE>(acc, a[rt][k], tf32_lo(b0), tf32_lo(b1));
+                                        mma<MODE>(acc, a[rt][k], tf32_hi(b0), tf32_hi(b1));
                                     } else {
                                         mma<MODE>(acc, a[rt][k], b0, b1);
                                     }
                                 }
+#pragma unroll
+                                for (int j = 0; j < 4; j++) to[j] = F::FOLD ? to[j] + acc[j] : acc[j];
+                            }
                         }
                     }
                 }
