@@ -150,21 +150,33 @@ __device__ __forceinline__ uint32_t bf16_pair_rn(float a, float b) {
 // hi pairs, then (two parts) 8 of lo pairs.
 template <class T, int D, int... I>
 __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t q, uint32_t k, uint32_t kind, std::integer_sequence<int, I...>) {
+    constexpr uint32_t part = T::PLANE >> 4;
+    constexpr bool CROSS = T::QP == 2 || T::VP == 2;
+    (([&] {   // the small products first: what the sum truncates is of their own size then
+         constexpr uint32_t o = ((I / 4) * 16384 + (I % 4) * 32) >> 4;
+         if constexpr (T::QP == 2) ptx::mma_f16_ss<o + part, o>(d, q, k, kind, I ? 1u : 0u);
+         if constexpr (T::VP == 2) ptx::mma_f16_ss<o, o + part>(d, q, k, kind, I || T::QP == 2 ? 1u : 0u);
+     }()),
+     ...);
     (([&] {
-         constexpr uint32_t o = ((I / 4) * 16384 + (I % 4) * 32) >> 4, part = T::PLANE >> 4;
-         ptx::mma_f16_ss<o, o>(d, q, k, kind, I ? 1u : 0u);
-         if constexpr (T::QP == 2) ptx::mma_f16_ss<o + part, o>(d, q, k, kind, 1u);
-         if constexpr (T::VP == 2) ptx::mma_f16_ss<o, o + part>(d, q, k, kind, 1u);
+         constexpr uint32_t o = ((I / 4) * 16384 + (I % 4) * 32) >> 4;
+         ptx::mma_f16_ss<o, o>(d, q, k, kind, I || CROSS ? 1u : 0u);
      }()),
      ...);
 }
 template <class T, int... I>
 __device__ __forceinline__ void issue_values(uint32_t d, uint32_t a, uint32_t v, uint32_t kind, uint32_t add, std::integer_sequence<int, I...>) {
+    constexpr uint32_t part = T::PLANE >> 4;
+    constexpr bool CROSS = T::QP == 2 || T::VP == 2;
     (([&] {
-         constexpr uint32_t o = I * 2048 >> 4, part = T::PLANE >> 4, col = I * 8 * T::QP;
-         ptx::mma_f16_ts<col, o>(d, a, v, kind, I ? 1u : add);
-         if constexpr (T::QP == 2) ptx::mma_f16_ts<col + 8, o>(d, a, v, kind, 1u);
-         if constexpr (T::VP == 2) ptx::mma_f16_ts<col, o + part>(d, a, v, kind, 1u);
+         constexpr uint32_t o = I * 2048 >> 4, col = I * 8 * T::QP;
+         if constexpr (T::QP == 2) ptx::mma_f16_ts<col + 8, o>(d, a, v, kind, I ? 1u : add);
+         if constexpr (T::VP == 2) ptx::mma_f16_ts<col, o + part>(d, a, v, kind, I || T::QP == 2 ? 1u : add);
+     }()),
+     ...);
+    (([&] {
+         constexpr uint32_t o = I * 2048 >> 4, col = I * 8 * T::QP;
+         ptx::mma_f16_ts<col, o>(d, a, v, kind, I || CROSS ? 1u : add);
      }()),
      ...);
 }
@@ -531,7 +543,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 if constexpr (T::DIRECT) ptx::fence_proxy_async_smem();   // the copies landed as ordinary writes
             };
             auto release = [&](int n) { ptx::mma_commit(&bar.empty[n % T::SLOTS]); };
-            auto scores = [&](int chain, int q_tile, int load) {   // S = Q.K^T: all features, hi.hi then the cross terms
+            auto scores = [&](int chain, int q_tile, int load) {   // S = Q.K^T: all features
                 issue_scores<T, D>(tmem + T::COL_S + chain * 128, q_desc + (uint32_t)(q_tile * (T::QP * T::PLANE >> 4)),
                                    k_desc + (uint32_t)(load % T::SLOTS * (T::SLOT >> 4)), kind_s, std::make_integer_sequence<int, D / 16>());
             };
