@@ -38,12 +38,14 @@
 //
 // Measured: 64 sequences of up to 8192 positions, one token each, 8 heads of
 // 128: int8 168 us = 3.8 TB/s, bf16 262 = 4.8, fp32 625 = 4.0; two of 131072
-// in bf16 211 us = 5.0 TB/s.  8-bit caches are bound by issue (copies in flight
-// cost as much as the products: a look-up and an address for each 128 bytes,
-// scales 4 bytes at a time), the others by loads in flight.  Drafted runs of 5
-// tokens x 4 heads (32 rows) over fp8 126 us: the rows' weights and fragments
-// are 4 times those of 8 rows.  One token over 200 positions in fp32 takes 14
-// us, a chain of 4300 instructions a warp.
+// in bf16 211 us = 5.0 TB/s.  8-bit caches are bound by the chain of dependent
+// instructions of three warps a scheduler (issue slots 44 % busy, DRAM 47 %;
+// the registers allow no fourth warp), and half of what is issued is the
+// copies: a look-up and an address for each 128 bytes, scales 4 bytes at a time;
+// the others are bound by loads in flight.  Drafted runs of 5 tokens x 4 heads
+// (32 rows) over fp8 126 us: the rows' weights and fragments are 4 times those
+// of 8 rows.  One token over 200 positions in fp32 takes 14 us, a chain of 4300
+// instructions a warp.
 #include <cuda_fp16.h>
 
 #include <algorithm>

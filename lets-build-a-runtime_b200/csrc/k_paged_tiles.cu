@@ -29,9 +29,9 @@
 // with bf16 outputs that is nothing even over long caches and O stays in TMEM,
 // with fp32 outputs every key tile's O is folded into fp32 registers.
 //
-// Bound: by the two products a 128 x 128 tile would take 1024 cycles at D = 128,
-// its 16384 exponentials 1024 as well.  Measured it is the softmax warps'
-// instruction issue: 4096 tokens over 16384 positions, 16 heads of 128, bf16,
+// Bound: the two products of a 128 x 128 tile take 1024 cycles at D = 128, its
+// 16384 exponentials 1024 as well.  Measured it is the softmax warps'
+// instructions: 4096 tokens over 16384 positions, 16 heads of 128, bf16,
 // 566 us = 850 TF/s (2700 cycles a tile); with a quarter of the exponentials
 // on the FMA pipe instead it takes 628 us, with waits that poll harder 574 -
 // 628.  fp32 activations have two products for one, two threads a row that
