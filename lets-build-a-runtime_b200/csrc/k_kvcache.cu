@@ -12,7 +12,7 @@
 // writing 16 K tokens of 8 heads of 128 from bf16 to fp8, 149 MB, 34 us = 4.4
 // TB/s, bound by the instructions of the quantisation and by loads in flight
 // (without the stores it takes as long; 4 loads a batch or a whole look-up per
-// thread 41 - 51); one token of 12 heads 4.9 us, one short prefix read 2.6.
+// thread 41 - 51); one token of 8 sequences 4.9 us, one short prefix read 2.6.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
