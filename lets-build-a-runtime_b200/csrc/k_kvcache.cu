@@ -353,13 +353,23 @@ RowMap row_map(const RtKvCache& c, int n_tokens, int most, dim3& grid, dim3& blo
     while ((1 << m.lanes_log2) < m.units) m.lanes_log2++;
     m.per_token = (2 * c.n_heads) << m.lanes_log2;
     const int chunks = (m.per_token + KV_THREADS - 1) / KV_THREADS;
-    const int x = chunks == 1 ? m.per_token : ((m.per_token + chunks - 1) / chunks + 31) / 32 * 32;
-    const int side = std::min(KV_THREADS / x, most);
+    int x = chunks == 1 ? m.per_token : ((m.per_token + chunks - 1) / chunks + 31) / 32 * 32;
+    int side = std::min(KV_THREADS / x, most);
+    // whole warps: by rows of threads without a token, or lanes without a part (5 heads of 16 in bf16
+    // are 20 lanes a token; the last warp of 5 tokens would have 4 lanes, and a token's place is
+    // fetched from the lane of the token's number)
+    int step = 1;
+    while (x * step % 32) step *= 2;
+    if ((side + step - 1) / step * step * x > KV_THREADS) {
+        x = (x + 31) / 32 * 32;
+        step = 1;
+        side = std::min(KV_THREADS / x, most);
+    }
     // `most` tokens a block for long calls, fewer when that would leave SMs without a block
     const int64_t fill = (int64_t)n_tokens * chunks / (2 * g_num_sms);
     m.tokens = std::max(side, (int)std::min<int64_t>(most, fill) / side * side);
     grid = dim3((unsigned)(((int64_t)n_tokens + m.tokens - 1) / m.tokens), chunks);
-    block = dim3(x, std::min(side, n_tokens));
+    block = dim3(x, (std::min(side, n_tokens) + step - 1) / step * step);
     m.page_shift = 0;
     while (((uint64_t)1 << m.page_shift) < (uint64_t)c.page_size) m.page_shift++;
     m.page_mul = (uint32_t)(((uint64_t)((((uint64_t)1 << m.page_shift) - c.page_size)) << 32) / c.page_size + 1);
