@@ -491,7 +491,8 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
 #pragma unroll
                             for (int k = 0; k < N; k++) x[k] = 0.0f;
                         }
-                        if (piece16 == 0) scales[r] = down;
+                        // (a row of zeros has scale 0: weights are as large as the other rows' scales are small)
+                        if (piece16 == 0) scales[r] = top[i] ? down : 0.0f;
                         if (finite && top[i]) top_all = max(top_all, __float_as_uint(down));
                         const uint32_t at = dst + place_of(at_row);
                         if constexpr (T::VP == 1) {

@@ -34,6 +34,32 @@ def owners(s):
     return [(b, n - m + i) for b, (n, m) in enumerate(zip(s.lens, s.new)) for i in range(m)]
 
 
+# ------------------------------------------------------------------ value rows of zeros
+@pytest.mark.parametrize("cache,act", CACHES)
+@pytest.mark.parametrize("dim,lens,new", [(64, [200, 90], [200, 60]), (128, [700], [100]), (64, [300], [1]), (64, [700] * 4, [100] * 4)])
+def test_value_rows_of_zeros(paged, cache, act, dim, lens, new):
+    """The first token's values or the first 300, scattered ones, and all of one head."""
+    hkv = 2 if len(lens) < 4 else 16                    # (several tiles in a row in a block)
+    s = Setup(cache, act, 2 * hkv, hkv, dim, 16, lens, new, seed=20)
+    for b, n in enumerate(lens):
+        for pos in [*range(1 if b % 2 == 0 else min(300, n)), *range(5, n, 7)]:
+            s.pages["v"][place(s, b, pos)] = 0
+            if s.scale["v"] is not None:
+                s.scale["v"][place(s, b, pos)] = 0      # as kv_write stores a row of zeros
+    for b, n in enumerate(lens):
+        for pos in range(n):
+            pg, off = place(s, b, pos)
+            s.pages["v"][pg, off, 1] = 0
+            if s.scale["v"] is not None:
+                s.scale["v"][pg, off, 1] = 0
+    lse = torch.empty(s.q.shape[:2], device="cuda")
+    out = s.attend(paged, lse=lse)
+    compare(s, out, act)
+    assert bool((out[:, 2:4] == 0).all())               # query heads of the head without values
+    _, want = s.expected()
+    assert float((lse.double() - want).abs().max()) < (1e-4 if act == "f32" else 2e-2)
+
+
 # ------------------------------------------------------------------ small heads in the cache
 @pytest.mark.parametrize("cache", ["f32", "bf16", "i8", "f8"])
 @pytest.mark.parametrize("act", ["f32", "bf16"])
