@@ -882,7 +882,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                             for (int i = 0; i < NO; i += 2) upk2(mul2(pk2(o[i], o[i + 1]), ff), o[i], o[i + 1]);
                         }
                         if (j >= 2) fold(t);
-                        ref_of[t] = ref;
+                        ref_of[t] = m == -INFINITY ? -INFINITY : ref;   // (nothing seen so far: O is 0, and the reference may come down)
                         weigh(x, wg * 64, tile_no, masked);
 #pragma unroll
                         for (int b = 0; b < 64; b += 16) {   // per 16 positions: 8 columns of hi pairs, 8 of lo pairs

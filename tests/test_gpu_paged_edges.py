@@ -60,6 +60,34 @@ def test_value_rows_of_zeros(paged, cache, act, dim, lens, new):
     assert float((lse.double() - want).abs().max()) < (1e-4 if act == "f32" else 2e-2)
 
 
+# ------------------------------------------------------------------ scores far below zero
+@pytest.mark.parametrize("cache,act", CACHES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_low_scores_under_a_window(paged, cache, act, dim):
+    """All scores near -150, rows of a tile that see nothing of its first keys.
+
+    A score is off by 2^-19 of |q||k| scale (bf16 activations: 2^-10, a q of one fp16 part), which
+    changes weights by as much and an output by at most twice that of the largest value.  There are
+    enough heads and sequences for several tiles in a row in a block."""
+    s = Setup(cache, act, 16, 16, dim, 16, [700, 300, 650, 512], [300] * 4, seed=24)
+    a = math.sqrt(150 / math.sqrt(dim))
+    s.q.copy_((a + 0.1 * s.q.float()).to(s.q.dtype))
+    k = -a + 0.1 * torch.randn(s.pages["k"].shape, generator=gen(25), device="cuda")
+    if s.scale["k"] is not None:
+        m = 448.0 if cache == "f8" else 127.0
+        s.scale["k"] = k.abs().amax(-1) / m
+        k = k / s.scale["k"][..., None]
+        k = k.round() if cache == "i8" else k
+    s.pages["k"] = k.to(CACHE[cache])
+    vmax = float(values(s.pages["v"], s.scale["v"]).nan_to_num(0, 0, 0).abs().max())
+    tol = 2 * 165 * 2.0 ** -19 * vmax if act == "f32" else (2 * 165 * 2.0 ** -10 + 2.0 ** -7) * vmax
+    for window in (200, 100):
+        out = s.attend(paged, window=window)
+        ref, _ = s.expected(window=window)
+        assert bool(out.isfinite().all())
+        assert float((out.double() - ref).abs().max()) <= tol
+
+
 # ------------------------------------------------------------------ small heads in the cache
 @pytest.mark.parametrize("cache", ["f32", "bf16", "i8", "f8"])
 @pytest.mark.parametrize("act", ["f32", "bf16"])
