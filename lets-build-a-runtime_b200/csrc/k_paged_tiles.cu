@@ -208,6 +208,12 @@ __device__ __forceinline__ Segment segment_of(const PagedArgs& p, const PagedCur
     return g;
 }
 
+// Do rows of the item see the key tile at k differently?
+__device__ __forceinline__ bool rows_differ(const PagedArgs& p, const Segment& g, const PagedSeq& s, int k) {
+    const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = s.L - s.n;
+    return tok1 > tok0 && ((p.a.causal && k + TKT > at0 + tok0 + 1) || (p.a.window > 0 && k < at0 + tok1 - p.a.window + 1));
+}
+
 template <int CT, bool F32ACT, int D>
 __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constant__ PagedArgs p) {
     using T = Tile<CT, F32ACT, D>;
@@ -319,10 +325,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             off_now = j & 1 ? off1 : off0;
             sp_now = j & 1 ? sp1 : sp0;
             live = __ballot_sync(0xffffffffu, off_now != ~0u);
-            if constexpr (T::DIRECT) {   // do rows of the item see this tile differently?
-                const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = cur.s.L - cur.s.n, k = g.k0 + j * TKT;
-                mixed = is_v && tok1 > tok0 && ((p.a.causal && k + TKT > at0 + tok0 + 1) || (p.a.window > 0 && k < at0 + tok1 - p.a.window + 1));
-            }
+            if constexpr (T::DIRECT) mixed = is_v && rows_differ(p, g, cur.s, g.k0 + j * TKT);
         };
         auto end_load = [&]() {
             n_copy++;
@@ -935,7 +938,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                             ptx::tmem_ld_wait();
                         }
                         const float top = see(x, 0, tile_no, k0, masked);
-                        if (!T::DIRECT || masked) {
+                        // values that are not finite were taken out of a tile that rows of the item see
+                        // differently, for the rows that see all of it too
+                        const bool noted = T::DIRECT && rows_differ(p, g, s, k0);
+                        if (!T::DIRECT || noted) {
                             wait_v(tile_no);
                             if (!ok) break;
                         }
@@ -967,7 +973,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                             ptx::tmem_st16(s_at + b / 2, w);
                         }
                         if constexpr (T::DIRECT) {
-                            if (masked) {   // values that are not finite were taken out: rows that see one get NaN
+                            if (noted) {   // rows that see such a value get NaN
                                 const uint32_t* sw = bar.strange[tile_no & 7];
                                 if (sw[0] | sw[1] | sw[2] | sw[3])
                                     for (int i = 0; i < TKT; i++)

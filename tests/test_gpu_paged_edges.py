@@ -60,6 +60,26 @@ def test_value_rows_of_zeros(paged, cache, act, dim, lens, new):
     assert float((lse.double() - want).abs().max()) < (1e-4 if act == "f32" else 2e-2)
 
 
+# ------------------------------------------------------------------ values that are not finite
+@pytest.mark.parametrize("cache,act", [("f32", "f32"), ("bf16", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("dim,new,window,back", [(d, n, w, b) for d, n, w in [(64, 300, 0), (128, 300, 0), (64, 300, 100), (128, 300, 100),
+                                                                              (64, 6, 0), (64, 6, 4)]
+                                                 for b in (1, 5, 40, 120, 239, 255, 299) if b <= n])
+def test_only_rows_that_see_a_value_get_it(paged, cache, act, dim, new, window, back):
+    """An infinite value `back` positions from the end: rows that see it are not finite, the rest are as without it."""
+    s = Setup(cache, act, 4, 2, dim, 16, [500], [new], seed=22)
+    ref, _ = s.expected(window=window)
+    pos = 500 - back
+    pg, off = place(s, 0, pos)
+    s.pages["v"][pg, off, 0, 3] = math.inf
+    out = s.attend(paged, window=window)
+    at = torch.arange(500 - new, 500, device="cuda")
+    hit = torch.zeros(s.q.shape[:2], dtype=torch.bool, device="cuda")
+    hit[:, :2] = ((at >= pos) & (at < pos + window if window else at >= 0))[:, None]
+    assert bool((~out.isfinite()).any(-1).eq(hit).all())
+    assert float((out.double() - ref)[~hit].abs().max()) <= tolerance(Setup(cache, act, 4, 2, dim, 16, [500], [new], seed=22), act)
+
+
 # ------------------------------------------------------------------ scores far below zero
 @pytest.mark.parametrize("cache,act", CACHES)
 @pytest.mark.parametrize("dim", [64, 128])
