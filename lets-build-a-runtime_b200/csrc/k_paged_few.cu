@@ -812,11 +812,10 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
                 float m = -INFINITY, ls = 0.0f, sum[4] = {0, 0, 0, 0};
                 for (int k = h; k < FW; k += p.head_group) m = fmaxf(m, ml[k * 2 * R + r]);
                 for (int k = h; k < FW; k += p.head_group) {
-                    const float mk = ml[k * 2 * R + r];
-                    if (mk == -INFINITY) continue;                             // (a warp without positions)
-                    const float f = exp2_fast(mk - m);
-                    if (f == 0.0f) continue;
-                    ls += ml[k * 2 * R + R + r] * f;
+                    const float lk = ml[k * 2 * R + R + r];
+                    if (lk == 0.0f) continue;                                  // (a warp that saw nothing)
+                    const float f = lk == lk ? exp2_fast(ml[k * 2 * R + r] - m) : lk;   // NaN scores: no maximum, a sum of NaN
+                    ls += lk * f;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const int n = (d + j) / (8 * F::VE) * F::VE + (d + j) % F::VE, col = (d + j) / F::VE % 8;

@@ -350,9 +350,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
         float ls = 0.0f;
         if (mine)
             for (int k = lane; k < n; k += LANES) {
-                const float x = factor[k * J::ROWS + lr], f = x == -INFINITY ? 0.0f : exp2_fast(x - m);
+                // a share that saw nothing has no weight and is left out; one whose scores are all
+                // NaN has no maximum, but a weight sum of NaN, which goes into the result
+                const float l = slot_of(k)[R * DP + R + first_row + lr];
+                const float f = l == 0.0f ? -1.0f : l == l ? exp2_fast(factor[k * J::ROWS + lr] - m) : l;
                 factor[k * J::ROWS + lr] = f;
-                ls += f == 0.0f ? 0.0f : slot_of(k)[R * DP + R + first_row + lr] * f;
+                ls += f < 0.0f ? 0.0f : l * f;
             }
         top[lr][lane] = ls;
         __syncthreads();
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
 #pragma unroll 8
                 for (int k = part; k < n; k += J::PARTS) {
                     const float f = factor[k * J::ROWS + r];
-                    const float4 x = f == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(slot_of(k) + (first_row + r) * DP + d);
+                    const float4 x = f < 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(slot_of(k) + (first_row + r) * DP + d);
                     sum[0] += x.x * f; sum[1] += x.y * f; sum[2] += x.z * f; sum[3] += x.w * f;
                 }
             }

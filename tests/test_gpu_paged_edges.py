@@ -60,6 +60,48 @@ def test_value_rows_of_zeros(paged, cache, act, dim, lens, new):
     assert float((lse.double() - want).abs().max()) < (1e-4 if act == "f32" else 2e-2)
 
 
+# ------------------------------------------------------------------ NaN scores
+@pytest.mark.parametrize("cache,act", CACHES)
+@pytest.mark.parametrize("lens,new,bounds", [
+    ([33], [1], {}),                                    # one block, a warp has the newest position to itself
+    ([33], [1], {"max_kv": 33, "max_new": 1}),
+    ([5000], [1], {"max_new": 1}),                      # cut over many blocks
+    ([400] * 70, [1] * 70, {"max_new": 1, "max_kv": 600}),   # a warp has a head to itself
+    ([2000, 300], [5, 60], {"max_new": 60}),            # tiles
+])
+def test_nan_queries_and_keys_give_nan(paged, cache, act, lens, new, bounds):
+    """softmax of a NaN score is NaN, and so is its log-sum-exp, however the work is split."""
+    def run(change):
+        s = Setup(cache, act, 4, 2, 64, 16, lens, new, seed=21)
+        ref, want = s.expected()
+        hit = change(s)                                 # [rows, query heads] that must be NaN
+        lse = torch.empty(s.q.shape[:2], device="cuda")
+        out = s.attend(paged, lse=lse, **bounds)
+        assert bool(out[hit].isnan().all()) and bool(lse[hit].isnan().all())
+        assert bool(out[~hit].isfinite().all()) and bool(lse[~hit].isfinite().all())
+        assert float((out.double() - ref)[~hit].abs().max()) <= tolerance(s, act)
+
+    def query(s):
+        hit = torch.zeros(s.q.shape[:2], dtype=torch.bool, device="cuda")
+        hit[::3, 1] = hit[0, 2] = True
+        s.q[hit] = math.nan
+        return hit
+
+    def newest_key(s):                                  # of cache head 1: query heads 2 and 3
+        for b, n in enumerate(s.lens):
+            pg, off = place(s, b, n - 1)
+            if s.scale["k"] is None:
+                s.pages["k"][pg, off, 1] = math.nan
+            else:
+                s.scale["k"][pg, off, 1] = math.nan
+        hit = torch.zeros(s.q.shape[:2], dtype=torch.bool, device="cuda")
+        for r, (b, pos) in enumerate(owners(s)):
+            hit[r, 2:] = pos == s.lens[b] - 1
+        return hit
+    run(query)
+    run(newest_key)
+
+
 # ------------------------------------------------------------------ values that are not finite
 @pytest.mark.parametrize("cache,act", [("f32", "f32"), ("bf16", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("dim,new,window,back", [(d, n, w, b) for d, n, w in [(64, 300, 0), (128, 300, 0), (64, 300, 100), (128, 300, 100),
