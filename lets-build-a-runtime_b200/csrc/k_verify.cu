@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
     bool residual = n < limit;
     const T* row = target + n * v.target_stride[1];
     const T* qrow = draft && residual ? draft + n * v.draft_stride[1] : nullptr;
-    const int point = !draft && residual ? v.draft_tokens[b * N + n] : -1;   // a certain draft: q is 1 there
+    int point = !draft && residual ? v.draft_tokens[b * N + n] : -1;   // a certain draft: q is 1 there
     const int lo = min(V, rank * slice), size = min(V, lo + slice) - lo, pieces = (size + C - 1) / C;
     row += lo;
     if (qrow) qrow += lo;
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
                     for (int k = 0; k < EACH; k++) {
                         const int i = from + k;
                         p[k] = 0.0f;
-                        q[k] = lo + i == point && residual ? 1.0f : 0.0f;
+                        q[k] = lo + i == point ? 1.0f : 0.0f;
                         if (i >= g_to) continue;
                         if (in_ring) {
                             const uint8_t* at = ring + (slot0 + i / C) % SLOTS * 2 * ROW_SLOT;
@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
             break;
         }
         residual = false;   // nothing left of the residual: the target's own row
+        point = -1;
     }
     if (rank == 0) {
         for (int i = t; i <= N; i += VT + 32)

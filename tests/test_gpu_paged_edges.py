@@ -150,6 +150,26 @@ def test_low_scores_under_a_window(paged, cache, act, dim):
         assert float((out.double() - ref).abs().max()) <= tol
 
 
+# ------------------------------------------------------------------ drafted tokens
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [9, 1000, 40000])
+def test_certain_draft_that_takes_all_the_mass(paged, act, V):
+    """A refused certain draft on a row whose only mass is its token: sampled from the target's row."""
+    target = torch.zeros(3, 3, V, device="cuda")
+    x = torch.tensor([[0, 1], [V - 1, 2], [V // 2, 3]], dtype=torch.int32, device="cuda")
+    for b in range(3):
+        target[b, 0, int(x[b, 0])] = 0.5
+        target[b, 1] = 1.0 / V
+    target = target.to(ACT[act])
+    au, su = torch.full((3, 2), 0.9, device="cuda"), torch.tensor([0.0, 0.5, 0.999], device="cuda")
+    got, acc = paged.verify_draft(target, None, x, au, su)
+    want, wacc = settle(target.float().cpu().numpy(), None, x.cpu().numpy(), au.cpu().numpy(), su.cpu().numpy())
+    np.testing.assert_array_equal(acc.cpu().numpy(), wacc)
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
+    assert got[:, 0].tolist() == x[:, 0].tolist()
+    paged.check_stream()
+
+
 # ------------------------------------------------------------------ small heads in the cache
 @pytest.mark.parametrize("cache", ["f32", "bf16", "i8", "f8"])
 @pytest.mark.parametrize("act", ["f32", "bf16"])
