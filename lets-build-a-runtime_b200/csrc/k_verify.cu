@@ -131,6 +131,8 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
     const T* target = static_cast<const T*>(v.target) + b * v.target_stride[0];
     const T* draft = v.draft ? static_cast<const T*>(v.draft) + b * v.draft_stride[0] : nullptr;
 
+    if (blocks > 1) ptx::cluster_started_arrive();
+
     // ---- how many drafts stand ----
     if (t == 0) {
         first = N;
@@ -238,6 +240,7 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
             group_sums[t] = x;
         }
         __syncthreads();
+        if (pass == 0 && blocks > 1) ptx::cluster_started_wait();   // (before the stores to other blocks)
         if (warp == 0) {
             unsigned long long mine = 0;
             for (int i = lane; i < groups; i += 32) mine += group_sums[i];

@@ -339,6 +339,14 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same in two steps: all blocks of the cluster have started once the wait
+// is over (before that their shared memory may not be touched).
+__device__ __forceinline__ void cluster_started_arrive() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_started_wait() {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 // Arrive on an mbarrier of any CTA of the cluster (shared::cluster address).
 // Default (CTA-scope release) semantics: the arrivals here only hand over
 // TMEM, which tcgen05 fences order; a cluster-scope release would first wait

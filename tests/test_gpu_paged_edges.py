@@ -170,6 +170,30 @@ def test_certain_draft_that_takes_all_the_mass(paged, act, V):
     paged.check_stream()
 
 
+@pytest.mark.parametrize("B", [1, 2, 19, 37, 74])
+def test_verify_while_other_work_holds_the_gpu(paged, B):
+    """A sequence's blocks exchange their sums wherever and whenever they get to run: the same answer next to
+    products on another stream that take SMs at other times."""
+    V = 20011
+    target = torch.softmax(2 * torch.randn(B, 3, V, generator=gen(33), device="cuda"), -1)
+    draft = torch.softmax(2 * torch.randn(B, 2, V, generator=gen(34), device="cuda"), -1)
+    x = torch.randint(0, V, (B, 2), generator=gen(35), device="cuda").to(torch.int32)
+    au, su = torch.rand(B, 2, generator=gen(36), device="cuda"), torch.rand(B, generator=gen(37), device="cuda")
+    want, wacc = settle(*(t.cpu().numpy() for t in (target, draft, x, au, su)))
+    side, a = torch.cuda.Stream(), torch.randn(1000, 1000, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    results = []
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            a = torch.tanh(a @ a)
+        results.append(paged.verify_draft(target, draft, x, au, su))
+    torch.cuda.current_stream().wait_stream(side)
+    paged.check_stream()
+    for got, acc in results:
+        np.testing.assert_array_equal(acc.cpu().numpy(), wacc)
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
 # ------------------------------------------------------------------ small heads in the cache
 @pytest.mark.parametrize("cache", ["f32", "bf16", "i8", "f8"])
 @pytest.mark.parametrize("act", ["f32", "bf16"])
