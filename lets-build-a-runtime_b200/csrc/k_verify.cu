@@ -80,6 +80,11 @@ __device__ __forceinline__ unsigned long long warp_scan(unsigned long long x, in
     return x;
 }
 
+// A wait of a whole warp: all its lanes go on, or none.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+    return __all_sync(0xffffffffu, ptx::wait_short(bar, parity, abort_flag, err, KERR_WAIT, WAIT_NS));
+}
+
 // Entries [0, size) of a row from `base` (any alignment) as pieces in a ring.
 template <class T>
 struct RowPieces {
@@ -179,6 +184,7 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
     unsigned long long total = 0;
     const int group_mask = (1 << group_shift) - 1;
     int slot = 0, phase = 0, slot0 = 0;   // slot0: the pass's first
+    int filled = 0;                       // slots filled so far, over both passes
     for (int pass = 0; pass < 2; pass++) {
         const bool two = residual && qrow;
         slot0 = slot;
@@ -186,7 +192,7 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
             for (int c = 0; c < pieces; c++) {
                 uint8_t* at = ring + slot * 2 * ROW_SLOT;
                 // (a slot's n-th filling waits for its (n - 1)-th emptying; the first for none)
-                ptx::wait_short(&empty[slot], phase ^ 1, &abort_flag, err, KERR_WAIT, WAIT_NS);
+                if (!wait_warp(&empty[slot], phase ^ 1, &abort_flag, err)) break;
                 uint32_t bytes = 0;
                 if (lane == 0) {
                     bytes = ps.copy(c, at, &full[slot]);
@@ -198,12 +204,13 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
                     __syncwarp();
                 }
                 if (lane == 0) ptx::mbar_expect_tx(&full[slot], bytes);
+                filled++;
                 if (++slot == SLOTS) slot = 0, phase ^= 1;
             }
         } else {
             uint32_t hi = 0, lo20 = 0;
             for (int c = 0; c < pieces; c++) {
-                ptx::wait_short(&full[slot], phase, &abort_flag, err, KERR_WAIT, WAIT_NS);
+                if (!wait_warp(&full[slot], phase, &abort_flag, err)) break;
                 const T* p = reinterpret_cast<const T*>(ring + slot * 2 * ROW_SLOT + ps.off) + t;
                 const T* q = reinterpret_cast<const T*>(ring + slot * 2 * ROW_SLOT + ROW_SLOT + qs.off) + t;
                 auto sum = [&](auto whole, auto with_q) {
@@ -357,6 +364,12 @@ __global__ void __launch_bounds__(VT + 32, BLOCKS_PER_SM) verify_kernel(const __
             if (i != n || !total) v.tokens[b * (N + 1) + i] = i < n ? v.draft_tokens[b * N + i] : -1;
         if (t == 0) v.accepted[b] = n;
     }
+    // after an abandoned wait the results mean nothing, but no copy may land here once the block is gone
+    if (warp == VT / 32 && lane == 0 && *static_cast<volatile int*>(&abort_flag))
+        for (int i = max(0, filled - SLOTS); i < filled; i++) {
+            volatile int no_abort = 0;
+            ptx::wait_bounded(&full[i % SLOTS], (i / SLOTS) & 1, &no_abort, err, KERR_WAIT, WAIT_NS);
+        }
 }
 
 template <class T>
