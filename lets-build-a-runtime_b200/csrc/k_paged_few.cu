@@ -534,7 +534,28 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             __syncwarp();
             copy_half();
             const uint32_t v_at = ring_at + slot * F::SLOT_BYTES;
-            const float* v_scale = reinterpret_cast<const float*>(ring + slot * F::SLOT_BYTES + F::HALF);
+            float* v_scale = reinterpret_cast<float*>(ring + slot * F::SLOT_BYTES + F::HALF);
+            if constexpr (CT == RT_F8E4M3) {
+                // Codes 0x7f and 0xff are NaN, and so is 0 times them. Where rows see different
+                // positions such a row of values becomes zeros with a scale of NaN.
+                if (mixed) {
+#pragma unroll 1
+                    for (int i = 0; i < F::VK * F::VC; i++) {
+                        uint32_t x[F::VB / 4], top = 0;
+                        const uint32_t at = (i * 32 + lane) * F::VB;
+                        read_part(x, v_at + at);
+#pragma unroll
+                        for (int k = 0; k < F::VB / 4; k++) top |= (x[k] & 0x7f7f7f7fu) + 0x01010101u;
+                        if (top & 0x80808080u) {
+                            const int n = i / F::VC;   // as the copies place rows
+#pragma unroll
+                            for (int k = 0; k < F::VB / 4; k++) reinterpret_cast<uint32_t*>(ring + slot * F::SLOT_BYTES + at)[k] = 0;
+                            v_scale[(n >> 2) * 16 + ((n >> 1) & 1) * 8 + 2 * t + (n & 1)] = __uint_as_float(0x7fc00000u);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
             slot = slot + 1 == F::SLOTS ? 0 : slot + 1;
             float to_w = 0.0f;
             if constexpr (F::Q8) {

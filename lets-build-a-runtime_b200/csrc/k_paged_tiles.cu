@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             off_now = j & 1 ? off1 : off0;
             sp_now = j & 1 ? sp1 : sp0;
             live = __ballot_sync(0xffffffffu, off_now != ~0u);
-            if constexpr (T::DIRECT) mixed = is_v && rows_differ(p, g, cur.s, g.k0 + j * TKT);
+            if constexpr (T::DIRECT || CT == RT_F8E4M3) mixed = is_v && rows_differ(p, g, cur.s, g.k0 + j * TKT);
         };
         auto end_load = [&]() {
             n_copy++;
@@ -400,14 +400,14 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             cp_wait<0>();
         } else {
             constexpr int AHEAD = T::NRAW - 1;
-            volatile uint32_t* meta = bar.meta[warp];       // by load & 7: is_v | tile << 1
+            volatile uint32_t* meta = bar.meta[warp];       // by load & 7: is_v | mixed << 1 | tile << 2
             volatile uint32_t* there = bar.there[warp];
             int part = 0, raw_c = 0;                        // piece of the load, raw slot
             auto copy_piece = [&]() {
                 if (part == 0) {
                     begin_load();
                     if (lane == 0) {
-                        meta[n_copy & 7] = (is_v ? 1u : 0u) | (uint32_t)tile_no << 1;
+                        meta[n_copy & 7] = (is_v ? 1u : 0u) | (mixed ? 2u : 0u) | (uint32_t)tile_no << 2;
                         there[n_copy & 7] = live;
                     }
                     if constexpr (T::Q8)
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             auto hand_piece = [&]() {
                 const uint32_t what = meta[n_done & 7];
                 const bool v = what & 1;
-                const int tile = (int)(what >> 1), s = n_done % T::SLOTS;
+                const int tile = (int)(what >> 2), s = n_done % T::SLOTS;
                 const uint32_t dst = ring + (uint32_t)s * T::SLOT, src = raw + (uint32_t)raw_d * T::RAW_PIECE;
                 float* scales = v ? reinterpret_cast<float*>(smem + T::OFF_VS) + tile % (T::DIRECT ? 1 : T::VSD) * 128
                                   : reinterpret_cast<float*>(smem + T::OFF_KS) + tile % (T::DIRECT ? 1 : T::KSD) * 128;
@@ -446,6 +446,23 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         const float scale = *reinterpret_cast<const volatile float*>(smem + T::OFF_RAW_SCALE + ((n_done & 7) * 128 + tid) * 4);
                         scales[tid] = scale;
                         if (scale > 0.0f && scale < INFINITY) top_all = __float_as_uint(scale);
+                    }
+                }
+                if constexpr (CT == RT_F8E4M3) {
+                    // Codes 0x7f and 0xff are NaN, and so is 0 times them. Where rows see the tile
+                    // differently such a row of values becomes zeros with a scale of NaN.
+                    if (what & 2u) {
+                        __syncwarp();   // (the scales are there)
+#pragma unroll
+                        for (int i = 0; i < PER; i++) {
+                            uint32_t top = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) top |= (w[i][k] & 0x7f7f7f7fu) + 0x01010101u;
+                            if (top & 0x80808080u) {
+                                w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0;
+                                scales[warp * 32 + (done_part * PER + i) * ROWS + sub_row] = __uint_as_float(0x7fc00000u);
+                            }
+                        }
                     }
                 }
                 if constexpr (T::Q8) {

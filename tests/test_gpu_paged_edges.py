@@ -122,6 +122,25 @@ def test_only_rows_that_see_a_value_get_it(paged, cache, act, dim, new, window, 
     assert float((out.double() - ref)[~hit].abs().max()) <= tolerance(Setup(cache, act, 4, 2, dim, 16, [500], [new], seed=22), act)
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("new,lens", [(6, 230), (6, 3000), (70, 230), (300, 500)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_codes_that_are_nan(paged, act, new, lens, which):
+    """Codes 0x7f / 0xff of an e4m3 cache at positions that only later rows see."""
+    s = Setup("f8", act, 4, 2, 64, 16, [lens], [new], seed=23)
+    ref, _ = s.expected()
+    pos = lens - 4
+    pg, off = place(s, 0, pos)
+    s.pages[which].view(torch.uint8)[pg, off, 0, 3] = 0x7f
+    s.pages[which].view(torch.uint8)[pg, off, 0, 60] = 0xff
+    out = s.attend(paged)
+    at = torch.arange(lens - new, lens, device="cuda")
+    hit = torch.zeros(s.q.shape[:2], dtype=torch.bool, device="cuda")
+    hit[:, :2] = (at >= pos)[:, None]
+    assert bool((~out.isfinite()).any(-1).eq(hit).all())
+    assert float((out.double() - ref)[~hit].abs().max()) <= tolerance(Setup("f8", act, 4, 2, 64, 16, [lens], [new], seed=23), act)
+
+
 # ------------------------------------------------------------------ scores far below zero
 @pytest.mark.parametrize("cache,act", CACHES)
 @pytest.mark.parametrize("dim", [64, 128])
