@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
             c_row[i] = base / up[i];
             m_ref[i] = -INFINITY;
             l[i] = 0.0f;
-            lo_row[i] = p.a.window > 0 ? max(0, at - p.a.window + 1) : 0;
+            lo_row[i] = paged_lo(p, at);
             hi_row[i] = p.a.causal ? max(0, min(s.L, at + 1)) : s.L;
             if (r < rows) {
                 all_lo = max(all_lo, lo_row[i]);

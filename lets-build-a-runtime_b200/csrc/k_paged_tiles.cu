@@ -211,7 +211,7 @@ __device__ __forceinline__ Segment segment_of(const PagedArgs& p, const PagedCur
 // Do rows of the item see the key tile at k differently?
 __device__ __forceinline__ bool rows_differ(const PagedArgs& p, const Segment& g, const PagedSeq& s, int k) {
     const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = s.L - s.n;
-    return tok1 > tok0 && ((p.a.causal && k + TKT > at0 + tok0 + 1) || (p.a.window > 0 && k < at0 + tok1 - p.a.window + 1));
+    return tok1 > tok0 && ((p.a.causal && k + TKT > at0 + tok0 + 1) || k < paged_lo(p, at0 + tok1));
 }
 
 template <int CT, bool F32ACT, int D>
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             const int my_row = g.row0 + row + (g.two ? wg * 128 : 0);
             const bool live = my_row < g.row0 + g.rows, any_live = __any_sync(0xffffffffu, live);
             const int at_pos = s.L - s.n + my_row / p.group;
-            const int lo_row = p.a.window > 0 ? max(0, at_pos - p.a.window + 1) : 0;
+            const int lo_row = paged_lo(p, at_pos);
             const int hi_row = live ? (p.a.causal ? min(s.L, at_pos + 1) : s.L) : 0;
             float c_row = base, m = -INFINITY, l = 0.0f, ref = 0.0f, v_top = 0.0f;   // ref: what exponents are taken against
             // Scores of N positions from b on: times their scales, -inf where the row does not see them; their maximum.

@@ -73,12 +73,17 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& p, int b) {
     return s;
 }
 
+// The first position that a token at `at` sees (at < 0: before the first; windows of any size).
+__device__ __forceinline__ int paged_lo(const PagedArgs& p, int at) {
+    return p.a.window > 0 && at >= p.a.window ? at - p.a.window + 1 : 0;
+}
+
 template <int R>
 __device__ __forceinline__ PagedTiles paged_tiles(const PagedArgs& p, const PagedSeq& s, int qt) {
     PagedTiles t;
     const int last = (min((qt + 1) * R, s.n * p.group) - 1) / p.group, first = qt * R / p.group;
     t.hi = p.a.causal ? min(s.L, s.L - s.n + last + 1) : s.L;
-    t.lo = p.a.window > 0 ? max(0, s.L - s.n + first - p.a.window + 1) : 0;
+    t.lo = paged_lo(p, s.L - s.n + first);
     if (t.lo >= t.hi) t.lo = t.hi = 0;
     t.t0 = t.lo >> p.key_shift;
     t.count = max(1, ((t.hi + (1 << p.key_shift) - 1) >> p.key_shift) - t.t0);

@@ -169,6 +169,15 @@ def test_low_scores_under_a_window(paged, cache, act, dim):
         assert float((out.double() - ref).abs().max()) <= tol
 
 
+# ------------------------------------------------------------------ windows as large as integers go
+@pytest.mark.parametrize("new", [7, 60])
+@pytest.mark.parametrize("causal", [True, False])
+def test_largest_window(paged, new, causal):
+    """More new tokens than positions, so that some stand before the first: a window that hides nothing."""
+    s = Setup("f32", "f32", 4, 2, 64, 16, [3, 40], [new, new], seed=28)
+    compare(s, s.attend(paged, window=2 ** 31 - 1, causal=causal), "f32", causal=causal)
+
+
 # ------------------------------------------------------------------ drafted tokens
 @pytest.mark.parametrize("act", ["f32", "bf16"])
 @pytest.mark.parametrize("V", [9, 1000, 40000])
