@@ -304,8 +304,10 @@ int rt_kv_read(const RtKvRead* r, void* stream);
  * or all of them, and with window > 0 only j > P - window.  out = softmax(q.k
  * * scale) v with query head h reading cache head h / (n_q_heads / n_heads);
  * lse (may be NULL, [tokens][n_q_heads]) = log of the softmax's sum.  A token
- * that sees nothing gets out = 0, lse = -inf.  Positions that no token of the
- * call sees are never read into the result, whatever they hold.
+ * that sees nothing gets out = 0, lse = -inf, and so does a row of q that
+ * belongs to no sequence (before cu_new[0], from cu_new[n_seqs] on, or of a
+ * sequence whose offsets are refused).  What a position holds that a token
+ * does not see never enters its result.
  * max_new / max_kv: the host's bounds on the per-sequence counts; they choose
  * how the work is split, not what is computed.  `ws` holds
  * rt_paged_attention_workspace(p) bytes of device memory, 16-byte aligned, used by

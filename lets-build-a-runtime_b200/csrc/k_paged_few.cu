@@ -206,8 +206,10 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
     asm volatile("griddepcontrol.launch_dependents;");
     PagedCursor cur;
     int u, per, total;
-    const bool some = paged_schedule<FT, R>(p, blockIdx.x, gridDim.x, sched, cur, u, per, total);
+    bool rest;
+    const bool some = paged_schedule<FT, R>(p, blockIdx.x, gridDim.x, sched, cur, u, per, total, rest);
     paged_note<R>(p, some, cur, u, per);
+    if (rest) paged_rest<FT>(p);
     if (!some) return;
     const int u_end = (int)min((int64_t)u + per, (int64_t)total);
 

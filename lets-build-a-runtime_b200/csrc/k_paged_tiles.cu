@@ -229,8 +229,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
     asm volatile("griddepcontrol.launch_dependents;");
     PagedCursor cur;
     int u, per, total;
-    const bool some = paged_schedule<TT, T::R>(p, blockIdx.x, gridDim.x, reinterpret_cast<int*>(smem), cur, u, per, total);
+    bool rest;
+    const bool some = paged_schedule<TT, T::R>(p, blockIdx.x, gridDim.x, reinterpret_cast<int*>(smem), cur, u, per, total, rest);
     paged_note<T::R>(p, some, cur, u, per);
+    if (rest) paged_rest<TT>(p);
     if (!some) return;
     const int u_end = (int)min((int64_t)u + per, (int64_t)total);
 

@@ -104,9 +104,40 @@ __device__ __forceinline__ int paged_units(const PagedArgs& p, const PagedSeq& s
     return sum * p.head_groups;
 }
 
+// `refused`: set where the sequence's offsets are refused.
 template <int R>
-__device__ __forceinline__ int paged_units(const PagedArgs& p, int b) {
-    return b >= p.a.n_seqs ? 0 : paged_units<R>(p, paged_seq(p, b));
+__device__ __forceinline__ int paged_units(const PagedArgs& p, int b, bool& refused) {
+    if (b >= p.a.n_seqs) return 0;
+    const PagedSeq s = paged_seq(p, b);
+    if (s.n == 0 && p.a.cu_new[b] != p.a.cu_new[b + 1]) refused = true;
+    return paged_units<R>(p, s);
+}
+
+// Zeros, and a log-sum-exp of -inf, for the rows of q that no sequence owns: padding before the
+// first and after the last sequence's, rows of a refused one.  A warp per row.
+template <int T>
+__device__ __forceinline__ void paged_rest(const PagedArgs& p) {
+    const int lane = threadIdx.x & 31, total = p.a.total_new, D = p.a.cache.head_dim;
+    for (int64_t row = (int64_t)blockIdx.x * (T / 32) + (threadIdx.x >> 5); row < total; row += (int64_t)gridDim.x * (T / 32)) {
+        bool owned = false;
+        for (int b = lane; b - lane < p.a.n_seqs && !owned; b += 32) {
+            bool mine = false;
+            if (b < p.a.n_seqs) {
+                const int first = p.a.cu_new[b], n = p.a.cu_new[b + 1] - first;
+                mine = first >= 0 && n >= 0 && n <= total - first && row >= first && row - first < n;
+            }
+            owned = __any_sync(0xffffffffu, mine);
+        }
+        if (owned) continue;
+        for (int h = 0; h < p.a.n_q_heads; h++) {
+            const int64_t at = row * p.a.out_stride[0] + h * p.a.out_stride[1];
+            for (int d = lane; d < D; d += 32) {
+                if (p.a.dtype == RT_BF16) static_cast<__nv_bfloat16*>(p.a.out)[at + d] = __float2bfloat16_rn(0.0f);
+                else static_cast<float*>(p.a.out)[at + d] = 0.0f;
+            }
+            if (p.a.lse && lane == 0) p.a.lse[row * p.a.n_q_heads + h] = -INFINITY;
+        }
+    }
 }
 
 // Inclusive sum over the block's T threads; `total` gets the block's sum.
@@ -160,11 +191,12 @@ struct PagedCursor {
     }
 };
 
-// The units of this call and the block's share.  `unit`: the first unit to
-// look at (c * per).  False when the block has none.  sh: T / 32 + 2 ints.
+// The units of this call and the block's share.  `u`: the first unit to
+// look at (c * per).  False when the block has none.  `rest`: some rows of q
+// belong to no sequence.  sh: T / 32 + 2 ints.
 template <int T, int R>
 __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, int blocks, int* sh, PagedCursor& c, int& u,
-                                               int& per, int& total) {
+                                               int& per, int& total, bool& rest) {
     auto settle = [&](int r) {   // row tile, then head group and key tile, from units after the sequence's first
         while (true) {
             const int per_head = p.whole ? 1 : c.t.count, n = per_head * p.head_groups;
@@ -182,6 +214,7 @@ __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, in
         PagedSeq s = {lane, 0, 0, 0};
         if (lane < p.a.n_seqs) s = paged_seq(p, lane);
         const int mine = s.n > 0 ? paged_units<R>(p, s) : 0;
+        rest = __reduce_add_sync(0xffffffffu, s.n) != p.a.total_new;
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -204,21 +237,23 @@ __device__ __forceinline__ bool paged_schedule(const PagedArgs& p, int block, in
         settle(r);
         return true;
     }
-    int mine = paged_units<R>(p, (int)threadIdx.x), all;
+    bool left = p.a.cu_new[0] != 0 || p.a.cu_new[p.a.n_seqs] != p.a.total_new;
+    int mine = paged_units<R>(p, (int)threadIdx.x, left), all;
     int incl = paged_scan<T>(mine, sh, &all);
     total = all;
     for (int base = T; base < p.a.n_seqs; base += T) {
         int part;
-        paged_scan<T>(paged_units<R>(p, base + (int)threadIdx.x), sh, &part);
+        paged_scan<T>(paged_units<R>(p, base + (int)threadIdx.x, left), sh, &part);
         total += part;
     }
+    rest = __syncthreads_or(left);
     per = max(p.min_units, (total + blocks - 1) / blocks);
     u = (int)min((int64_t)block * per, (int64_t)0x7fffffff);
     if (u >= total) return false;
     int carry = 0;
     for (int base = 0;; base += T) {
         if (base) {
-            mine = paged_units<R>(p, base + (int)threadIdx.x);
+            mine = paged_units<R>(p, base + (int)threadIdx.x, left);
             incl = paged_scan<T>(mine, sh, &all);
         }
         const int first = carry + incl - mine;

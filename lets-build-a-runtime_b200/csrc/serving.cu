@@ -89,7 +89,7 @@ Status check_rows(const void* p, const int64_t st[2], int64_t rows, int heads, i
 
 Status check_table(const int* table, int64_t stride, int width, int n_seqs) {
     if (width < 0 || stride < 0) return bad("page_table: negative width or stride");
-    if (width == 0) return Status::ok();
+    if (width == 0 || n_seqs == 0) return Status::ok();
     return check_pointer(table, (size_t)((n_seqs - 1) * stride + width) * 4, "page_table");
 }
 
@@ -136,7 +136,7 @@ Status do_attention(const RtPagedAttention& p, void* ws, size_t ws_bytes, void* 
     t_checked = p.cache.flags & RT_POINTERS_CHECKED;
     CHECK(check_attention_sizes(p));
     CHECK(check_cache(p.cache));
-    if (p.total_new == 0 || p.n_seqs == 0) return Status::ok();
+    if (p.total_new == 0) return Status::ok();   // (without sequences every row is written as zeros)
     const int D = p.cache.head_dim;
     CHECK(check_rows(p.q, p.q_stride, p.total_new, p.n_q_heads, D, p.dtype, "paged_attention q"));
     CHECK(check_rows(p.out, p.out_stride, p.total_new, p.n_q_heads, D, p.dtype, "paged_attention out"));
@@ -144,7 +144,7 @@ Status do_attention(const RtPagedAttention& p, void* ws, size_t ws_bytes, void* 
         return bad("paged_attention: rows of out overlap");
     if (p.lse) CHECK(check_pointer(p.lse, (size_t)p.total_new * p.n_q_heads * 4, "paged_attention lse"));
     CHECK(check_table(p.page_table, p.table_stride, p.table_width, p.n_seqs));
-    CHECK(check_pointer(p.kv_lens, (size_t)p.n_seqs * 4, "paged_attention kv_lens"));
+    if (p.n_seqs) CHECK(check_pointer(p.kv_lens, (size_t)p.n_seqs * 4, "paged_attention kv_lens"));
     CHECK(check_pointer(p.cu_new, (size_t)(p.n_seqs + 1) * 4, "paged_attention cu_new"));
     const size_t need = paged_attention_workspace(p);
     if (ws_bytes < need) return bad("paged_attention: workspace of " + std::to_string(ws_bytes) + " bytes, needs " + std::to_string(need));

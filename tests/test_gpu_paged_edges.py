@@ -169,6 +169,58 @@ def test_low_scores_under_a_window(paged, cache, act, dim):
         assert float((out.double() - ref).abs().max()) <= tol
 
 
+# ------------------------------------------------------------------ rows and sequences nobody owns
+@pytest.mark.parametrize("cache,act", [("f32", "f32"), ("bf16", "bf16"), ("i8", "f32")])
+@pytest.mark.parametrize("seqs,new", [(3, 1), (40, 1), (3, 50), (40, 20)])
+def test_rows_without_a_sequence_are_zero(paged, cache, act, seqs, new):
+    """Padding before the first and after the last sequence's tokens."""
+    lens = [50 + 3 * i for i in range(seqs)]
+    s = Setup(cache, act, 4, 2, 64, 16, lens, [new] * seqs, seed=26)
+    ref, _ = s.expected()
+    n = len(s.q)
+    q = torch.randn(n + 12, 4, 64, device="cuda").to(ACT[act])
+    q[5:5 + n] = s.q
+    out = torch.full_like(q, 7.0)
+    lse = torch.full(q.shape[:2], 7.0, device="cuda")
+    paged.paged_attention(q, s.pages["k"], s.pages["v"], s.table, s.lens_t, s.cu + 5, **s.kw(), out=out, lse=lse)
+    paged.check_stream()
+    assert float((out[5:5 + n].double() - ref).abs().max()) <= tolerance(s, act)
+    pad = torch.ones(n + 12, dtype=torch.bool, device="cuda")
+    pad[5:5 + n] = False
+    assert bool((out[pad] == 0).all()) and bool((lse[pad] == -math.inf).all())
+    assert bool(lse[~pad].isfinite().all())
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("seqs", [3, 40])
+def test_rows_of_a_refused_sequence_are_zero(paged, new, seqs):
+    """Offsets past the end of q: the sequence is left out and reported, its rows are zeros."""
+    from lbr_b200.executor import CudaRuntimeError
+    s = Setup("f32", "f32", 4, 2, 64, 16, [60] * seqs, [new] * seqs, seed=27)
+    ref, _ = s.expected()
+    cu = s.cu.clone()
+    cu[-1] += 100
+    out = torch.full_like(s.q, 7.0)
+    lse = torch.full(s.q.shape[:2], 7.0, device="cuda")
+    paged.check_stream()
+    paged.paged_attention(s.q, s.pages["k"], s.pages["v"], s.table, s.lens_t, cu, out=out, lse=lse)
+    with pytest.raises(CudaRuntimeError, match="out of range"):
+        paged.check_stream()
+    assert bool((out[-new:] == 0).all()) and bool((lse[-new:] == -math.inf).all())
+    assert float((out[:-new].double() - ref[:-new]).abs().max()) <= tolerance(s, "f32")
+
+
+def test_attention_without_sequences(paged):
+    pages = torch.randn(3, 16, 2, 64, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    table, cu = torch.zeros(0, 4, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    for n in (1, 9, 100):
+        out, lse = torch.full((n, 4, 64), 7.0, device="cuda"), torch.full((n, 4), 7.0, device="cuda")
+        paged.paged_attention(torch.randn(n, 4, 64, device="cuda"), pages, pages, table, none, cu, out=out, lse=lse)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    paged.check_stream()
+
+
 # ------------------------------------------------------------------ windows as large as integers go
 @pytest.mark.parametrize("new", [7, 60])
 @pytest.mark.parametrize("causal", [True, False])
