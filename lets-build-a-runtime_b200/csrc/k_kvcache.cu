@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_consta
             }
         }
         const int first = r.cu[lo];
-        if (row < r.cu[r.n_seqs]) {
+        if (r.n_seqs > 0 && row < r.cu[r.n_seqs]) {
             const int64_t pos = (r.start ? r.start[lo] : 0) + (int64_t)(row - first);
             if (pos < 0 || pos >= min((int64_t)r.table_width * c.page_size, (int64_t)0x7fffffff) || row < first) {
                 atomicCAS(err, 0, KERR_LENGTH);

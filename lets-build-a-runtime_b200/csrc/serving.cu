@@ -111,11 +111,11 @@ Status do_read(const RtKvRead& r, void* stream) {
     CHECK(check_act(r.dtype));
     CHECK(check_cache(r.cache));
     if (r.n_rows < 0 || r.n_seqs < 0) return bad("kv_read: negative n_rows or n_seqs");
-    if (r.n_rows == 0 || r.n_seqs == 0) return Status::ok();
+    if (r.n_rows == 0) return Status::ok();   // (without sequences every row is written as zeros)
     CHECK(check_rows(r.k_out, r.k_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read k_out"));
     CHECK(check_rows(r.v_out, r.v_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read v_out"));
     CHECK(check_table(r.page_table, r.table_stride, r.table_width, r.n_seqs));
-    if (r.start) CHECK(check_pointer(r.start, (size_t)r.n_seqs * 4, "kv_read start"));
+    if (r.start && r.n_seqs) CHECK(check_pointer(r.start, (size_t)r.n_seqs * 4, "kv_read start"));
     CHECK(check_pointer(r.cu, (size_t)(r.n_seqs + 1) * 4, "kv_read cu"));
     DeviceGuard g;
     return launch_kv_read(r, static_cast<cudaStream_t>(stream));

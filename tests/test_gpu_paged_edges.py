@@ -221,6 +221,17 @@ def test_attention_without_sequences(paged):
     paged.check_stream()
 
 
+def test_read_without_sequences(paged):
+    pages = torch.randn(3, 16, 2, 64, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    table, cu = torch.zeros(0, 4, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    for start in (None, none):
+        k, v = torch.full((9, 2, 64), 7.0, device="cuda"), torch.full((9, 2, 64), 7.0, device="cuda")
+        paged.kv_read(pages, pages, table, start, cu, 9, out=(k, v))
+        assert bool((k == 0).all()) and bool((v == 0).all())
+    paged.check_stream()
+
+
 # ------------------------------------------------------------------ windows as large as integers go
 @pytest.mark.parametrize("new", [7, 60])
 @pytest.mark.parametrize("causal", [True, False])
