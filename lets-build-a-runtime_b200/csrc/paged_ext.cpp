@@ -39,11 +39,12 @@ void check(int code) {
     if (code) throw Status{code};
 }
 
-std::string shape_of(const at::Tensor& t) {
+std::string text_of(at::IntArrayRef x) {
     std::string s = "[";
-    for (int64_t i = 0; i < t.dim(); i++) s += (i ? ", " : "") + std::to_string(t.size(i));
+    for (size_t i = 0; i < x.size(); i++) s += (i ? ", " : "") + std::to_string(x[i]);
     return s + "]";
 }
+std::string shape_of(const at::Tensor& t) { return text_of(t.sizes()); }
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) type_error(std::string(name) + " must be a tensor");
@@ -85,11 +86,11 @@ void* stream() { return c10::cuda::getCurrentCUDAStream(g_device).stream(); }
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type) {
     return at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, g_device));
 }
-void* index(const at::Tensor& t, const char* name, int64_t n, at::ScalarType type) {
+void* index(const at::Tensor& t, const char* name, at::IntArrayRef shape, at::ScalarType type) {
     if (t.scalar_type() != type) type_error(std::string(name) + " must be " + toString(type) + ", got " + toString(t.scalar_type()));
     on_device(t, name);
-    if (t.numel() != n || !t.is_contiguous())
-        value_error(std::string(name) + " must be contiguous with " + std::to_string(n) + " elements, got " + shape_of(t));
+    if (t.sizes() != shape || !t.is_contiguous())
+        value_error(std::string(name) + " must be contiguous " + text_of(shape) + ", got " + (t.sizes() == shape ? "strided " : "") + text_of(t.sizes()));
     return t.data_ptr();
 }
 // A dense [a, b, c] operand with contiguous innermost dimension.
@@ -201,7 +202,7 @@ PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         w.k = k.data_ptr();
         w.v = v.data_ptr();
         w.n_tokens = narrow(tokens, "tokens");
-        w.slots = static_cast<const int64_t*>(index(slots, "slots", tokens, at::kLong));
+        w.slots = static_cast<const int64_t*>(index(slots, "slots", {tokens}, at::kLong));
         check(rt_kv_write(&w, stream()));
         Py_RETURN_NONE;
     });
@@ -234,8 +235,8 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         r.n_rows = narrow(total, "total");
         r.n_seqs = narrow(seqs, "cu");
         page_table(r, tensor(a[2], "page_table"), seqs);
-        if (const at::Tensor* start = optional(a[3], "start")) r.start = static_cast<const int*>(index(*start, "start", seqs, at::kInt));
-        r.cu = static_cast<const int*>(index(cu, "cu", seqs + 1, at::kInt));
+        if (const at::Tensor* start = optional(a[3], "start")) r.start = static_cast<const int*>(index(*start, "start", {seqs}, at::kInt));
+        r.cu = static_cast<const int*>(index(cu, "cu", {seqs + 1}, at::kInt));
         check(rt_kv_read(&r, stream()));
         return pair(k, v);
     });
@@ -259,11 +260,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.out = out.data_ptr();
         p.total_new = narrow(tokens, "tokens");
         p.n_q_heads = narrow(heads, "heads");
-        if (const at::Tensor* lse = optional(a[14], "lse")) p.lse = static_cast<float*>(index(*lse, "lse", tokens * heads, at::kFloat));
+        if (const at::Tensor* lse = optional(a[14], "lse")) p.lse = static_cast<float*>(index(*lse, "lse", {tokens, heads}, at::kFloat));
         p.n_seqs = narrow(lens.numel(), "kv_lens");
         page_table(p, tensor(a[3], "page_table"), p.n_seqs);
-        p.kv_lens = static_cast<const int*>(index(lens, "kv_lens", p.n_seqs, at::kInt));
-        p.cu_new = static_cast<const int*>(index(tensor(a[5], "cu_new"), "cu_new", p.n_seqs + 1, at::kInt));
+        p.kv_lens = static_cast<const int*>(index(lens, "kv_lens", {p.n_seqs}, at::kInt));
+        p.cu_new = static_cast<const int*>(index(tensor(a[5], "cu_new"), "cu_new", {p.n_seqs + 1}, at::kInt));
         if (a[8] == Py_None) {
             p.scale = 1.0f / sqrtf((float)dim);
         } else {
@@ -304,10 +305,10 @@ PyObject* verify_draft(PyObject*, PyObject* const* a, Py_ssize_t n) {
             rows(*draft, "draft", B, N, V, v.draft_stride);
             v.draft = draft->data_ptr();
         }
-        v.draft_tokens = static_cast<const int*>(index(tensor(a[2], "draft_tokens"), "draft_tokens", B * N, at::kInt));
-        v.accept_u = static_cast<const float*>(index(tensor(a[3], "accept_u"), "accept_u", B * N, at::kFloat));
-        v.sample_u = static_cast<const float*>(index(tensor(a[4], "sample_u"), "sample_u", B, at::kFloat));
-        if (const at::Tensor* lens = optional(a[5], "draft_lens")) v.draft_lens = static_cast<const int*>(index(*lens, "draft_lens", B, at::kInt));
+        v.draft_tokens = static_cast<const int*>(index(tensor(a[2], "draft_tokens"), "draft_tokens", {B, N}, at::kInt));
+        v.accept_u = static_cast<const float*>(index(tensor(a[3], "accept_u"), "accept_u", {B, N}, at::kFloat));
+        v.sample_u = static_cast<const float*>(index(tensor(a[4], "sample_u"), "sample_u", {B}, at::kFloat));
+        if (const at::Tensor* lens = optional(a[5], "draft_lens")) v.draft_lens = static_cast<const int*>(index(*lens, "draft_lens", {B}, at::kInt));
         const at::Tensor tokens = empty({B, N + 1}, at::kInt), accepted = empty({B}, at::kInt);
         v.tokens = static_cast<int*>(tokens.data_ptr());
         v.accepted = static_cast<int*>(accepted.data_ptr());

@@ -314,3 +314,41 @@ def test_write_of_tokens_that_fill_no_warp(paged, cache, act, heads, dim, n):
         top = x.abs().amax(-1, keepdim=True)
         tol = top / 127 * 0.5001 if cache == "i8" else torch.maximum(x.abs() * 2.0 ** -4, top / 448 * 2.0 ** -10) * 1.0001
         assert bool(((got[slots] * sc[slots][..., None] - x).abs() <= tol + x.abs() * 2.0 ** -22).all())
+
+
+# ------------------------------------------------------------------ shapes
+def test_refusals_by_shape(paged):
+    """Operands of the right number of elements in another order or shape."""
+    s = Setup("f32", "f32", 4, 2, 64, 16, [40, 50], [3, 3], seed=30)
+    kp, vp, q = s.pages["k"], s.pages["v"], s.q
+
+    def attend(**kw):
+        a = {"kv_lens": s.lens_t, "cu_new": s.cu, **kw}
+        return paged.paged_attention(q, kp, vp, s.table, a.pop("kv_lens"), a.pop("cu_new"), **a)
+    attend()
+    with pytest.raises(ValueError, match="lse"):
+        attend(lse=torch.empty(4, 6, device="cuda"))
+    with pytest.raises(ValueError, match="lse"):
+        attend(lse=torch.empty(24, device="cuda"))
+    with pytest.raises(ValueError, match="kv_lens"):
+        attend(kv_lens=s.lens_t[:, None])
+    with pytest.raises(ValueError, match="cu_new"):
+        attend(cu_new=s.cu[None])
+    i32 = {"dtype": torch.int32, "device": "cuda"}
+    with pytest.raises(ValueError, match="slots"):
+        paged.kv_write(s.k, s.v, kp, vp, torch.zeros(2, 3, dtype=torch.int64, device="cuda"))
+    with pytest.raises(ValueError, match="start"):
+        paged.kv_read(kp, vp, s.table, torch.zeros(2, 1, **i32), s.cu, 6)
+    with pytest.raises(ValueError, match="cu"):
+        paged.kv_read(kp, vp, s.table, None, s.cu[:, None], 6)
+    p, x, u = torch.rand(2, 4, 50, device="cuda"), torch.zeros(2, 3, **i32), torch.rand(2, 3, device="cuda")
+    paged.verify_draft(p, p[:, :3], x, u, u[:, 0].contiguous())
+    with pytest.raises(ValueError, match="draft_tokens"):
+        paged.verify_draft(p, p[:, :3], x.view(3, 2), u, u[:, 0].contiguous())
+    with pytest.raises(ValueError, match="accept_u"):
+        paged.verify_draft(p, p[:, :3], x, u.view(3, 2), u[:, 0].contiguous())
+    with pytest.raises(ValueError, match="sample_u"):
+        paged.verify_draft(p, p[:, :3], x, u, u[:, :1].contiguous())
+    with pytest.raises(ValueError, match="draft_lens"):
+        paged.verify_draft(p, p[:, :3], x, u, u[:, 0].contiguous(), draft_lens=torch.zeros(2, 1, **i32))
+    paged.check_stream()
