@@ -87,6 +87,13 @@ Status check_rows(const void* p, const int64_t st[2], int64_t rows, int heads, i
     return check_pointer(p, (size_t)span(rows, st[0], heads, st[1], dim) * e, what);
 }
 
+// What a call writes: rows that would fall on one another are refused.
+Status check_out(const void* p, const int64_t st[2], int64_t rows, int heads, int dim, int dtype, const char* what) {
+    CHECK(check_rows(p, st, rows, heads, dim, dtype, what));
+    if ((heads > 1 && st[1] < dim) || (rows > 1 && st[0] < dim)) return bad(std::string(what) + ": rows overlap");
+    return Status::ok();
+}
+
 Status check_table(const int* table, int64_t stride, int width, int n_seqs) {
     if (width < 0 || stride < 0) return bad("page_table: negative width or stride");
     if (width == 0 || n_seqs == 0) return Status::ok();
@@ -112,8 +119,8 @@ Status do_read(const RtKvRead& r, void* stream) {
     CHECK(check_cache(r.cache));
     if (r.n_rows < 0 || r.n_seqs < 0) return bad("kv_read: negative n_rows or n_seqs");
     if (r.n_rows == 0) return Status::ok();   // (without sequences every row is written as zeros)
-    CHECK(check_rows(r.k_out, r.k_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read k_out"));
-    CHECK(check_rows(r.v_out, r.v_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read v_out"));
+    CHECK(check_out(r.k_out, r.k_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read k_out"));
+    CHECK(check_out(r.v_out, r.v_stride, r.n_rows, r.cache.n_heads, r.cache.head_dim, r.dtype, "kv_read v_out"));
     CHECK(check_table(r.page_table, r.table_stride, r.table_width, r.n_seqs));
     if (r.start && r.n_seqs) CHECK(check_pointer(r.start, (size_t)r.n_seqs * 4, "kv_read start"));
     CHECK(check_pointer(r.cu, (size_t)(r.n_seqs + 1) * 4, "kv_read cu"));
@@ -139,9 +146,7 @@ Status do_attention(const RtPagedAttention& p, void* ws, size_t ws_bytes, void* 
     if (p.total_new == 0) return Status::ok();   // (without sequences every row is written as zeros)
     const int D = p.cache.head_dim;
     CHECK(check_rows(p.q, p.q_stride, p.total_new, p.n_q_heads, D, p.dtype, "paged_attention q"));
-    CHECK(check_rows(p.out, p.out_stride, p.total_new, p.n_q_heads, D, p.dtype, "paged_attention out"));
-    if ((p.n_q_heads > 1 && p.out_stride[1] < D) || (p.total_new > 1 && p.out_stride[0] < D))
-        return bad("paged_attention: rows of out overlap");
+    CHECK(check_out(p.out, p.out_stride, p.total_new, p.n_q_heads, D, p.dtype, "paged_attention out"));
     if (p.lse) CHECK(check_pointer(p.lse, (size_t)p.total_new * p.n_q_heads * 4, "paged_attention lse"));
     CHECK(check_table(p.page_table, p.table_stride, p.table_width, p.n_seqs));
     if (p.n_seqs) CHECK(check_pointer(p.kv_lens, (size_t)p.n_seqs * 4, "paged_attention kv_lens"));

@@ -352,3 +352,14 @@ def test_refusals_by_shape(paged):
     with pytest.raises(ValueError, match="draft_lens"):
         paged.verify_draft(p, p[:, :3], x, u, u[:, 0].contiguous(), draft_lens=torch.zeros(2, 1, **i32))
     paged.check_stream()
+
+
+def test_read_refuses_rows_that_overlap(paged):
+    from lbr_b200.executor import CudaRuntimeError
+    s = Setup("f32", "f32", 2, 2, 64, 16, [40], [3], seed=31)
+    one = torch.zeros(1, 2, 64, device="cuda")
+    with pytest.raises(CudaRuntimeError, match="overlap"):
+        paged.kv_read(s.pages["k"], s.pages["v"], s.table, None, s.cu, 3, out=(one.expand(3, 2, 64), one.expand(3, 2, 64)))
+    heads = torch.zeros(3, 1, 64, device="cuda")
+    with pytest.raises(CudaRuntimeError, match="overlap"):
+        paged.kv_read(s.pages["k"], s.pages["v"], s.table, None, s.cu, 3, out=(torch.zeros(3, 2, 64, device="cuda"), heads.expand(3, 2, 64)))
