@@ -59,6 +59,14 @@ int64_t integer(PyObject* o, const char* name) {
     }
     return v;
 }
+bool truth(PyObject* o, const char* name) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {   // an array of several, say
+        PyErr_Clear();
+        type_error(std::string(name) + " must be true or false");
+    }
+    return v;
+}
 int narrow(int64_t v, const char* name) {
     if (v < INT32_MIN || v > INT32_MAX) value_error(std::string(name) + " does not fit 32 bits");
     return (int)v;
@@ -274,7 +282,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 type_error("scale must be a number");
             }
         }
-        p.causal = PyObject_IsTrue(a[9]) == 1;
+        p.causal = truth(a[9], "causal");
         p.window = narrow(integer(a[10], "window"), "window");
         p.max_new = a[11] == Py_None ? p.total_new : narrow(integer(a[11], "max_new"), "max_new");
         const int64_t width = (int64_t)p.table_width * p.cache.page_size;

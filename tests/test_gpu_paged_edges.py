@@ -363,3 +363,9 @@ def test_read_refuses_rows_that_overlap(paged):
     heads = torch.zeros(3, 1, 64, device="cuda")
     with pytest.raises(CudaRuntimeError, match="overlap"):
         paged.kv_read(s.pages["k"], s.pages["v"], s.table, None, s.cu, 3, out=(torch.zeros(3, 2, 64, device="cuda"), heads.expand(3, 2, 64)))
+
+
+def test_causal_must_have_a_truth_value(paged):
+    s = Setup("f32", "f32", 2, 2, 64, 16, [40], [3], seed=32)
+    with pytest.raises(TypeError, match="causal"):
+        s.attend(paged, causal=np.ones(2))
