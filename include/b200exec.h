@@ -222,7 +222,8 @@ int rt_matmul_noalloc(const float* a, const float* b, const float* bias, float* 
  * checked on the host before anything is enqueued.  What only the device can
  * see (slots, page numbers, lengths, offsets) is bounds-checked by the
  * kernels: an entry out of range is treated as absent and reported as
- * RT_ERR_OUT_OF_RANGE by the next rt_check_stream / rt_synchronize. */
+ * RT_ERR_OUT_OF_RANGE by the next rt_check_stream (of whichever stream: the
+ * serving calls share one error word, which planned graphs do not see). */
 enum RtDtype { RT_F32 = 0, RT_BF16 = 1, RT_F8E4M3 = 2, RT_I8 = 3 };
 /* The caller has established that every pointer of the call is memory of the
  * library's device and spans what the sizes and strides say (a tensor library

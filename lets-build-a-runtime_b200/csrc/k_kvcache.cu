@@ -386,7 +386,7 @@ Status write_as(const RtKvWrite& w, cudaStream_t st) {
     const RowMap m = row_map<A>(w.cache, w.n_tokens, WRITE_TOKENS, grid, block);
     const bool vec = vector_rows(w.k, w.k_stride, w.dtype) && vector_rows(w.v, w.v_stride, w.dtype);
     if (grid.y > 65535) return Status::err(RT_ERR_UNSUPPORTED, "kv_write: too many heads");
-    kv_write_kernel<A, CT><<<grid, block, 0, st>>>(w, m, vec, kernel_error_flag());
+    kv_write_kernel<A, CT><<<grid, block, 0, st>>>(w, m, vec, serving_error_flag());
     RT_LAUNCH_CHECK();
     return Status::ok();
 }
@@ -396,7 +396,7 @@ Status read_as(const RtKvRead& r, cudaStream_t st) {
     const RowMap m = row_map<A>(r.cache, r.n_rows, READ_TOKENS, grid, block);
     const bool vec = vector_rows(r.k_out, r.k_stride, r.dtype) && vector_rows(r.v_out, r.v_stride, r.dtype);
     if (grid.y > 65535) return Status::err(RT_ERR_UNSUPPORTED, "kv_read: too many heads");
-    kv_read_kernel<A, CT><<<grid, block, 0, st>>>(r, m, vec, kernel_error_flag());
+    kv_read_kernel<A, CT><<<grid, block, 0, st>>>(r, m, vec, serving_error_flag());
     RT_LAUNCH_CHECK();
     return Status::ok();
 }

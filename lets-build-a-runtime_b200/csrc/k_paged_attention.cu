@@ -28,7 +28,7 @@ size_t paged_attention_workspace(const RtPagedAttention& p) {
 Status launch_paged_attention(const RtPagedAttention& a, void* ws, cudaStream_t st) {
     PagedArgs p{};
     p.a = a;
-    p.err = kernel_error_flag();
+    p.err = serving_error_flag();
     p.group = a.n_q_heads / a.cache.n_heads;
     p.vec_q = paged_rows16(a.q, a.q_stride, a.dtype);
     p.vec_out = paged_rows16(a.out, a.out_stride, a.dtype);

@@ -394,7 +394,7 @@ Status verify_as(const RtVerifyDraft& v, cudaStream_t st) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T>, v, blocks, slice, group_shift, kernel_error_flag()));
+    RT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T>, v, blocks, slice, group_shift, serving_error_flag()));
     return Status::ok();
 }
 

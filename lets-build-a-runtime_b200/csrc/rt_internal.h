@@ -232,11 +232,14 @@ int runtime_device();
 int report(const Status& s);   // records a failure for rt_last_error and returns its code
 // Device memory of the initialised device, `bytes` of it where the allocation is ours.
 Status check_device_pointer(const void* p, size_t bytes, const char* what);
-// After a synchronise: what a kernel left in the error word, as a status.
+// After a synchronise: what a planned graph's kernel, or a serving call's, left
+// in its error word, as a status.
 Status kernel_status();
+Status serving_status();
 int* kernel_error_flag();
-// Codes of the error word: 0x400.. an index read from device memory was out
-// of range, everything else an abandoned wait.
+int* serving_error_flag();
+// Codes of the serving calls' word: 0x400.. an index read from device memory
+// was out of range, everything else an abandoned wait.
 constexpr int KERR_SLOT = 0x401, KERR_PAGE = 0x402, KERR_LENGTH = 0x403, KERR_TOKEN = 0x404;
 constexpr int KERR_RANGE_FIRST = 0x400, KERR_RANGE_LAST = 0x4ff;
 

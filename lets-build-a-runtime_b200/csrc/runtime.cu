@@ -64,7 +64,7 @@ struct State {
     int last_error = RT_OK;
     std::string last_msg;
     std::vector<std::pair<uintptr_t, size_t>> protect;   // graph outputs (rt_protect)
-    volatile int* kerr_host = nullptr;   // host-mapped error word written by kernels
+    volatile int* kerr_host = nullptr;   // host-mapped error words written by kernels
     int* kerr_dev = nullptr;
     std::vector<cudaStream_t> chunk_streams;   // rt_execute_chunks, created on first use
 };
@@ -626,27 +626,37 @@ bool is_constant_range(const void* p, size_t bytes) {
     return a && a->constant;
 }
 
+// Two words: what planned graphs' kernels report and what the serving calls'
+// do, so that neither's mistake is returned by the other's calls.
+constexpr int SERVING_WORD = 8;   // (32 bytes from the first)
 int* kernel_error_flag() { return S().kerr_dev; }
+int* serving_error_flag() { return S().kerr_dev ? S().kerr_dev + SERVING_WORD : nullptr; }
 
 // After a synchronise: a kernel that gave up a bounded wait left its code.
-int take_kernel_error() {
+int take_error(int word) {
     if (!S().kerr_host) return 0;
-    int v = *S().kerr_host;
-    if (v) *S().kerr_host = 0;
+    volatile int* at = S().kerr_host + word;
+    int v = *at;
+    if (v) *at = 0;
     return v;
 }
 
-Status kernel_status() {
-    const int k = take_kernel_error();
-    if (!k) return Status::ok();
-    if (k >= KERR_RANGE_FIRST && k <= KERR_RANGE_LAST) {
-        const char* what = k == KERR_SLOT     ? "a cache slot"
-                           : k == KERR_PAGE   ? "a page number"
-                           : k == KERR_LENGTH ? "a sequence length or offset"
-                                              : "a drafted token";
-        return Status::err(RT_ERR_OUT_OF_RANGE, std::string(what) + " in device memory was out of range");
-    }
+Status wait_abandoned(int k) {
     return Status::err(RT_ERR_KERNEL_TIMEOUT, "a kernel abandoned a bounded wait, code " + std::to_string(k));
+}
+Status kernel_status() {
+    const int k = take_error(0);
+    return k ? wait_abandoned(k) : Status::ok();
+}
+Status serving_status() {
+    const int k = take_error(SERVING_WORD);
+    if (!k) return Status::ok();
+    if (k < KERR_RANGE_FIRST || k > KERR_RANGE_LAST) return wait_abandoned(k);
+    const char* what = k == KERR_SLOT     ? "a cache slot"
+                       : k == KERR_PAGE   ? "a page number"
+                       : k == KERR_LENGTH ? "a sequence length or offset"
+                                          : "a drafted token";
+    return Status::err(RT_ERR_OUT_OF_RANGE, std::string(what) + " in device memory was out of range");
 }
 
 bool runtime_ready() { return S().initialized; }

@@ -228,7 +228,7 @@ int rt_check_stream(void* stream) {
     return guarded([&] {
         cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) return Status::err(RT_ERR_CUDA, std::string("stream: ") + cudaGetErrorString(e));
-        return kernel_status();
+        return serving_status();
     });
 }
 

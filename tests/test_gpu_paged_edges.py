@@ -316,6 +316,28 @@ def test_write_of_tokens_that_fill_no_warp(paged, cache, act, heads, dim, n):
         assert bool(((got[slots] * sc[slots][..., None] - x).abs() <= tol + x.abs() * 2.0 ** -22).all())
 
 
+# ------------------------------------------------------------------ what one caller's mistake does to others
+def test_a_bad_slot_does_not_fail_planned_work(paged):
+    from lbr_b200.copnode import COpNode
+    from lbr_b200.executor import CudaRuntimeError, load_library
+    lib = load_library()
+    x = torch.zeros(1, 4, 64, device="cuda")
+    pages = torch.zeros(2, 16, 4, 64, device="cuda")
+    paged.kv_write(x, x, pages, pages.clone(), torch.zeros(1, dtype=torch.int64, device="cuda"))
+    paged.check_stream()
+    paged.kv_write(x, x, pages, pages.clone(), torch.tensor([10 ** 6], device="cuda"))
+    torch.cuda.synchronize()
+    arr = (COpNode * 1)()                               # one GELU of 256 elements
+    arr[0].op, arr[0].n_inputs, arr[0].n_dims, arr[0].elem_size = 104, 1, 1, 4
+    arr[0].inputs[0], arr[0].output = lib.rt_alloc(1024), lib.rt_alloc(1024)
+    arr[0].out_shape[0] = 256
+    assert lib.rt_execute(arr, 1, 0) == 0
+    assert lib.rt_synchronize() == 0
+    with pytest.raises(CudaRuntimeError, match="slot"):
+        paged.check_stream()
+    paged.check_stream()
+
+
 # ------------------------------------------------------------------ shapes
 def test_refusals_by_shape(paged):
     """Operands of the right number of elements in another order or shape."""
