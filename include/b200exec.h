@@ -95,7 +95,9 @@ typedef struct RtCopy {
 /* ---- lifecycle ---------------------------------------------------------- */
 /* Select the device, create the stream.  Idempotent for the same device. */
 int rt_init(int device);
-/* Free every allocation, cached plan and graph; the library may be re-inited. */
+/* Wait for the device, free every allocation, cached plan and graph; the
+ * library may be re-inited.  A caller's CUDA graphs that hold serving calls
+ * are not to be launched any more. */
 int rt_destroy(void);
 const char* rt_version(void);
 

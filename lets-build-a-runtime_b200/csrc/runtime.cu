@@ -733,11 +733,14 @@ int rt_init(int device) {
 int rt_destroy(void) {
     RT_GUARD;
     if (!S().initialized) return RT_OK;
-    cudaStreamSynchronize(S().stream);
-    for (cudaStream_t st : S().chunk_streams) {
-        cudaStreamSynchronize(st);
-        cudaStreamDestroy(st);
-    }
+    // All of the device: serving calls run on their callers' streams and may
+    // still report into the error words that are freed here.
+    int before = -1;
+    cudaGetDevice(&before);
+    cudaSetDevice(S().device);
+    cudaDeviceSynchronize();
+    if (before >= 0) cudaSetDevice(before);
+    for (cudaStream_t st : S().chunk_streams) cudaStreamDestroy(st);
     S().chunk_streams.clear();
     clear_plans();
     for (auto& kv : S().allocs) {

@@ -391,3 +391,38 @@ def test_causal_must_have_a_truth_value(paged):
     s = Setup("f32", "f32", 2, 2, 64, 16, [40], [3], seed=32)
     with pytest.raises(TypeError, match="causal"):
         s.attend(paged, causal=np.ones(2))
+
+
+# ------------------------------------------------------------------ the library's life
+def in_a_process(code):
+    import pathlib
+    import subprocess
+    import sys
+    root = pathlib.Path(__file__).resolve().parents[1]
+    head = ("import torch, sys\n"
+            f"sys.path.insert(0, {str(root)!r})\n"
+            "import __graft_entry__\n"
+            "__graft_entry__.load_package()\n"
+            "from lbr_b200 import paged\n"
+            "from lbr_b200.executor import CudaRuntimeError, load_library\n"
+            "lib = load_library()\n"
+            "x, p = torch.ones(2, 4, 64, device='cuda'), torch.zeros(3, 16, 4, 64, device='cuda')\n"
+            "write = lambda *at: paged.kv_write(x, x, p, p.clone(), torch.tensor(at, device='cuda'))\n")
+    r = subprocess.run([sys.executable, "-c", head + code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_destroy_waits_for_serving_calls(paged):
+    """Calls still under way on the caller's stream, with something to report, when the library ends."""
+    in_a_process("write(1, 2)\n"
+                 "a = torch.randn(4000, 4000, device='cuda')\n"
+                 "side = torch.cuda.Stream()\n"
+                 "torch.cuda.synchronize()\n"
+                 "with torch.cuda.stream(side):\n"
+                 "    at = torch.tensor([10 ** 6, 10 ** 7], device='cuda')\n"
+                 "    for _ in range(20): a = torch.tanh(a @ a)\n"
+                 "    paged.kv_write(x, x, p, p, at)\n"
+                 "assert lib.rt_destroy() == 0\n"
+                 "assert side.query()\n"
+                 "assert lib.rt_init(0) == 0\n"
+                 "torch.cuda.synchronize()\n")
