@@ -78,13 +78,15 @@ int act_code(const at::Tensor& t, const char* name) {
     type_error(std::string(name) + " must be float32 or bfloat16, got " + toString(t.scalar_type()));
 }
 
-// The library on this tensor's device (chosen by the first call of the process).
+// The library on this device (chosen by the first call, of the process or after
+// rt_destroy; does nothing where it runs there already).
+void use_device(int device) {
+    check(rt_init(device));
+    g_device = device;
+}
 void use_device(const at::Tensor& t, const char* name) {
     if (!t.is_cuda()) value_error(std::string(name) + " must be a CUDA tensor");
-    if (t.get_device() != g_device) {
-        check(rt_init(t.get_device()));
-        g_device = t.get_device();
-    }
+    use_device(t.get_device());
 }
 void on_device(const at::Tensor& t, const char* name) {
     if (!t.is_cuda() || t.get_device() != g_device)
@@ -332,11 +334,7 @@ PyObject* verify_draft(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* check_stream(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!count(n, 1)) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int device = narrow(integer(a[0], "device"), "device");
-        if (device != g_device) {
-            check(rt_init(device));
-            g_device = device;
-        }
+        use_device(narrow(integer(a[0], "device"), "device"));
         int code;
         void* st = stream();
         Py_BEGIN_ALLOW_THREADS;

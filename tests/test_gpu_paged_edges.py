@@ -426,3 +426,18 @@ def test_destroy_waits_for_serving_calls(paged):
                  "assert side.query()\n"
                  "assert lib.rt_init(0) == 0\n"
                  "torch.cuda.synchronize()\n")
+
+
+def test_calls_after_destroy_start_the_library_again(paged):
+    in_a_process("write(1, 2)\n"
+                 "paged.check_stream()\n"
+                 "assert lib.rt_destroy() == 0\n"
+                 "write(3, 4)\n"
+                 "paged.check_stream()\n"
+                 "write(3, 10 ** 6)\n"
+                 "try:\n"
+                 "    paged.check_stream()\n"
+                 "except CudaRuntimeError as e:\n"
+                 "    assert 'slot' in str(e)\n"
+                 "else:\n"
+                 "    raise SystemExit('nothing reported')\n")
