@@ -209,9 +209,7 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
     bool rest;
     const bool some = paged_schedule<FT, R>(p, blockIdx.x, gridDim.x, sched, cur, u, per, total, rest);
     paged_note<R>(p, some, cur, u, per);
-    if (rest) paged_rest<FT>(p);
-    if (!some) return;
-    const int u_end = (int)min((int64_t)u + per, (int64_t)total);
+    const int u_end = some ? (int)min((int64_t)u + per, (int64_t)total) : u;
 
     while (u < u_end) {
         const int seg = p.whole ? cur.t.count : min(cur.t.count - cur.i, u_end - u);
@@ -860,6 +858,9 @@ __global__ void __launch_bounds__(FT, R == 32 ? 2 : 3) paged_few_kernel(const __
         u += p.whole ? 1 : seg;
         cur.next_item<R>(p);
     }
+    // (here, and not above, the code is no longer on the way of a cold call: one token over 200
+    // positions 14.6 us against 15.4)
+    if (rest) paged_rest<FT>(p);
 }
 
 constexpr int MAX_BLOCKS_PER_SM = 3;
