@@ -196,6 +196,9 @@ struct Segment {
     int tiles, k0;        // key tiles, first position of the first
     int row0, rows;       // rows of the item
     bool two;             // chains have rows of their own
+    int all_lo, all_hi;   // positions that every row of the item sees
+    // Do rows of the item see the key tile at k differently?
+    __device__ __forceinline__ bool differ(int k) const { return k < all_lo || k + TKT > all_hi; }
 };
 template <class T>
 __device__ __forceinline__ Segment segment_of(const PagedArgs& p, const PagedCursor& c, int u, int u_end) {
@@ -205,13 +208,10 @@ __device__ __forceinline__ Segment segment_of(const PagedArgs& p, const PagedCur
     g.row0 = c.qt * T::R;
     g.rows = min(T::R, c.s.n * p.group - g.row0);
     g.two = T::R == 256 && g.rows > 128;
+    const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = c.s.L - c.s.n;
+    g.all_lo = tok1 > tok0 ? paged_lo(p, at0 + tok1) : 0;   // (a single token: all alike)
+    g.all_hi = tok1 > tok0 && p.a.causal ? at0 + tok0 + 1 : 0x7fffffff;
     return g;
-}
-
-// Do rows of the item see the key tile at k differently?
-__device__ __forceinline__ bool rows_differ(const PagedArgs& p, const Segment& g, const PagedSeq& s, int k) {
-    const int tok0 = g.row0 / p.group, tok1 = (g.row0 + g.rows - 1) / p.group, at0 = s.L - s.n;
-    return tok1 > tok0 && ((p.a.causal && k + TKT > at0 + tok0 + 1) || k < paged_lo(p, at0 + tok1));
 }
 
 template <int CT, bool F32ACT, int D>
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             off_now = j & 1 ? off1 : off0;
             sp_now = j & 1 ? sp1 : sp0;
             live = __ballot_sync(0xffffffffu, off_now != ~0u);
-            if constexpr (T::DIRECT || CT == RT_F8E4M3) mixed = is_v && rows_differ(p, g, cur.s, g.k0 + j * TKT);
+            if constexpr (T::DIRECT || CT == RT_F8E4M3) mixed = is_v && g.differ(g.k0 + j * TKT);
         };
         auto end_load = [&]() {
             n_copy++;
@@ -959,7 +959,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         const float top = see(x, 0, tile_no, k0, masked);
                         // values that are not finite were taken out of a tile that rows of the item see
                         // differently, for the rows that see all of it too
-                        const bool noted = T::DIRECT && rows_differ(p, g, s, k0);
+                        const bool noted = T::DIRECT && g.differ(k0);
                         if (!T::DIRECT || noted) {
                             wait_v(tile_no);
                             if (!ok) break;
