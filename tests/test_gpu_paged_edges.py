@@ -441,3 +441,77 @@ def test_calls_after_destroy_start_the_library_again(paged):
                  "    assert 'slot' in str(e)\n"
                  "else:\n"
                  "    raise SystemExit('nothing reported')\n")
+
+
+# ------------------------------------------------------------------ how good bf16 outputs are
+@pytest.mark.parametrize("cache", ["f32", "bf16", "i8", "f8"])
+@pytest.mark.parametrize("hq,hkv,dim,lens,new", [
+    (4, 2, 128, [3001, 700], [1, 1]),                   # few rows, over many blocks
+    (8, 2, 64, [9000], [5]),                            # a drafted run
+    (4, 2, 128, [2500], [300]),                         # tiles, two row tiles an item
+    (2, 2, 64, [4000, 130], [60, 100]),                 # tiles, alternate key tiles
+])
+def test_bf16_outputs_are_as_good_as_their_weights(paged, cache, hq, hkv, dim, lens, new):
+    """Weights w_j in bf16 are off by e_j, |e_j| <= 2^-8 of them and of either sign, evenly spread: an output
+    by sum w_j e_j v_j, whose standard deviation is at most 2^-8 / sqrt(3) sqrt(sum w_j^2 v_j^2); six of them,
+    the output's own rounding (2^-8 of it), and 2^-18 of the largest value for scores and sums.  That is little
+    enough to notice a key tile that is left out, which a bound by the largest value is not."""
+    s = Setup(cache, "bf16", hq, hkv, dim, 16, lens, new, seed=40)
+    out = s.attend(paged, max_new=max(new), max_kv=max(lens)).double()
+    group, r0 = hq // hkv, 0
+    for b, (n, m) in enumerate(zip(lens, new)):
+        pos = torch.arange(n, device="cuda")
+        pg, off = s.table[b].long()[pos // 16], pos % 16
+        k, v = (values(s.pages[x], s.scale[x])[pg, off].repeat_interleave(group, 1) for x in "kv")
+        z = torch.einsum("qhd,khd->hqk", s.q[r0:r0 + m].double(), k) * dim ** -0.5
+        z = z.masked_fill(pos > torch.arange(n - m, n, device="cuda")[:, None], -math.inf)
+        w = torch.softmax(z, -1)
+        want = torch.einsum("hqk,khd->qhd", w, v)
+        spread = torch.einsum("hqk,khd->qhd", w * w, v * v).sqrt()
+        tol = 2.0 ** -8 * (want.abs() + 6 / 3 ** 0.5 * spread) + 2.0 ** -18 * v.abs().max()
+        got = out[r0:r0 + m]
+        assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+        if n > 256:
+            z[..., 128:256] = -math.inf                 # a tile lost
+            lost = torch.einsum("hqk,khd->qhd", torch.softmax(z, -1), v)
+            assert not bool(((got - lost).abs() <= tol).all(0).all(0).any())
+        r0 += m
+
+
+# ------------------------------------------------------------------ graphs
+@pytest.mark.parametrize("cache,act,hq,lens,new", [("i8", "f32", 8, [3000, 90], [1, 1]), ("bf16", "bf16", 8, [700, 300], [200, 40]),
+                                                   ("f8", "bf16", 16, [2000] * 40, [3] * 40)])
+def test_calls_of_two_launches_in_a_graph(paged, cache, act, hq, lens, new):
+    """Write, attention that is cut over blocks and joined, and verification by clusters, captured once and
+    replayed on other contents."""
+    s = Setup(cache, act, hq, 4, 64, 16, lens, new, seed=41)
+    slots = torch.cat([s.table[b].long()[p // 16] * 16 + p % 16
+                       for b, (n, m) in enumerate(zip(lens, new)) for p in [torch.arange(n - m, n, device="cuda")]])
+    V = 30011
+    target = torch.softmax(2 * torch.randn(3, 3, V, generator=gen(42), device="cuda"), -1)
+    draft = torch.softmax(2 * torch.randn(3, 2, V, generator=gen(43), device="cuda"), -1)
+    x = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    au, su = torch.rand(3, 2, device="cuda"), torch.rand(3, device="cuda")
+    out = torch.empty_like(s.q)
+
+    def calls():
+        paged.kv_write(s.k, s.v, s.pages["k"], s.pages["v"], slots, **s.kw())
+        s.attend(paged, max_new=max(new), max_kv=max(lens), out=out)
+        return paged.verify_draft(target, draft, x, au, su)
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tokens, accepted = calls()
+    for i in range(3):
+        for t in (s.q, s.k, s.v):
+            t.copy_(torch.randn(t.shape, generator=gen(50 + i), device="cuda"))
+        x.copy_(torch.randint(0, V, x.shape, generator=gen(60 + i), device="cuda"))
+        au.uniform_(0, 1, generator=gen(70 + i))
+        out.fill_(7.0)
+        graph.replay()
+        paged.check_stream()
+        compare(s, out, act)
+        want, wacc = settle(*(t.cpu().numpy() for t in (target, draft, x, au, su)))
+        np.testing.assert_array_equal(accepted.cpu().numpy(), wacc)
+        np.testing.assert_array_equal(tokens.cpu().numpy(), want)
