@@ -236,7 +236,7 @@ enum RtDtype { RT_F32 = 0, RT_BF16 = 1, RT_F8E4M3 = 2, RT_I8 = 3 };
 /* One layer's cache, owned by the caller.  Element d of head h in slot s of
  * page p is k[p*stride[0] + s*stride[1] + h*stride[2] + d] (v alike); the
  * features are contiguous, k, v and the strides (in bytes) multiples of 16,
- * head_dim a multiple of 16 up to 128.  RT_F32 / RT_BF16 hold the values;
+ * the strides the same for k and v, head_dim a multiple of 16 up to 128.  RT_F32 / RT_BF16 hold the values;
  * RT_F8E4M3 / RT_I8 hold codes, and the value is code * scale with one scale
  * per (page, slot, head) at k_scale[p*scale_stride[0] + s*scale_stride[1] +
  * h*scale_stride[2]] (NULL otherwise). */
@@ -311,6 +311,8 @@ int rt_kv_read(const RtKvRead* r, void* stream);
  * belongs to no sequence (before cu_new[0], from cu_new[n_seqs] on, or of a
  * sequence whose offsets are refused).  What a position holds that a token
  * does not see never enters its result.
+ * A call's work is counted in tiles of at least 8 rows (new token, query head
+ * of a cache head) x 32 positions, fewer than 2^31 of them.
  * max_new / max_kv: the host's bounds on the per-sequence counts; they choose
  * how the work is split, not what is computed.  `ws` holds
  * rt_paged_attention_workspace(p) bytes of device memory, 16-byte aligned, used by

@@ -30,13 +30,18 @@
 // with fp32 outputs every key tile's O is folded into fp32 registers.
 //
 // Bound: the two products of a 128 x 128 tile take 1024 cycles at D = 128, its
-// 16384 exponentials 1024 as well.  Measured it is the softmax warps'
-// instructions: 4096 tokens over 16384 positions, 16 heads of 128, bf16,
-// 566 us = 850 TF/s (2700 cycles a tile); with a quarter of the exponentials
-// on the FMA pipe instead it takes 628 us, with waits that poll harder 574 -
-// 628.  fp32 activations have two products for one, two threads a row that
-// exchange their maximum, and weights in two parts: 12 heads of 64 over int8,
-// chunks of up to 1400 tokens, 497 us = 153 TF/s of plain products.
+// 16384 exponentials 1024 as well.  Measured it is neither, but the chain of a
+// tile: 4096 tokens over 16384 positions, 16 heads of 128, bf16, 530 us = 907
+// TF/s (2500 cycles a tile).  P lies over S, so the next scores of a chain wait
+// for all of its weights and then for all of P.V; of 4 warps a scheduler 0.5
+// could issue on average (2048 tokens over 8192: tensor pipe busy 43 %, issue
+// slots 36 %, exponential unit 38 %).  With a quarter of the exponentials on the
+// FMA pipe instead it was slower (566 -> 628 us when measured), and with waits
+// that poll harder (574 - 628).  fp32 activations have two products for one, two
+// threads a row that exchange their maximum, and weights in two parts: 12 heads
+// of 64 over int8, chunks of up to 1400 tokens, 495 us = 154 TF/s of plain
+// products (chunks of 700: tensor pipe 25 %, issue slots 41 %).  128 registers a
+// thread at launch cost every instance 400 - 700 bytes of spills.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -988,6 +993,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                             uint32_t w[16];
 #pragma unroll
                             for (int i = 0; i < 16; i++)
+                                // one part, whose rounding (2^-8, 2^-11) the sum averages: below the output's own
                                 w[i] = T::DIRECT ? bf16_pair_rn(x[b + 2 * i], x[b + 2 * i + 1]) : f16x2_rn(x[b + 2 * i], x[b + 2 * i + 1]);
                             ptx::tmem_st16(s_at + b / 2, w);
                         }

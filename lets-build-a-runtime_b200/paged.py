@@ -84,8 +84,8 @@ def _calls():
 def kv_write(k, v, k_pages, v_pages, slots, *, k_scale=None, v_scale=None) -> None:
     """Store the keys and values ``[tokens, heads, head_dim]`` of new tokens in a cache.
 
-    ``k_pages`` / ``v_pages``: ``[pages, page_size, heads, head_dim]`` (any strides with contiguous
-    features on 16-byte boundaries); ``slots``: int64 ``[tokens]``, ``page * page_size + position in
+    ``k_pages`` / ``v_pages``: ``[pages, page_size, heads, head_dim]`` (any strides, the same for both,
+    with contiguous features on 16-byte boundaries); ``slots``: int64 ``[tokens]``, ``page * page_size + position in
     the page``, negative to skip a token.  int8 and float8_e4m3fn caches take ``k_scale`` /
     ``v_scale``, float32 ``[pages, page_size, heads]``, and are written with one scale per token and
     head: ``scale = max|x| * (1/M)``, ``code = round(x * ((1/max|x|) * M))``, M = 127 or 448.
@@ -99,7 +99,7 @@ def kv_read(k_pages, v_pages, page_table, start, cu, total, *, k_scale=None, v_s
 
     Row ``cu[b] + i`` is position ``start[b] + i`` of sequence b (``start`` None: from 0); ``cu``:
     int32 ``[sequences + 1]``, ``total`` = its last value as the host knows it.  ``out``: a pair of
-    tensors to write instead of new ones of ``dtype`` (float32 / bfloat16).
+    tensors to write instead of new ones of ``dtype`` (float32 / bfloat16).  Rows past the last sequence's are zeros.
     """
     if dtype not in _dtypes:
         raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
@@ -116,7 +116,8 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, cu_new, *, k_scale
     positions, its new tokens' own included (write them first); ``page_table``: int32 ``[sequences,
     pages]``.  New token i of n stands at ``kv_lens[b] - n + i`` and sees what is at or before it
     (``causal``) and less than ``window`` positions back (0: no window).  Query head h reads cache head
-    ``h // (query heads / cache heads)``.  A token that sees nothing gives zeros.
+    ``h // (query heads / cache heads)``.  A token that sees nothing gives zeros, and so does a row of ``q``
+    that no sequence owns (before ``cu_new[0]``, from ``cu_new[-1]`` on).
 
     ``scale``: default 1/sqrt(head_dim).  ``max_new`` / ``max_kv``: the host's bounds on new and cached
     tokens of a sequence (default: the tokens of q, the width of the table); they only choose how the
@@ -143,5 +144,5 @@ def verify_draft(target, draft, draft_tokens, accept_u, sample_u, *, draft_lens=
 
 
 def check_stream(device=0) -> None:
-    """Wait for torch's current stream on `device` and raise for what its kernels reported."""
+    """Wait for torch's current stream on `device` and raise for what serving calls reported (of all streams)."""
     (_module or _calls()).check_stream(device if isinstance(device, int) else device.index)
