@@ -31,8 +31,8 @@
 //
 // Bound: the two products of a 128 x 128 tile take 1024 cycles at D = 128, its
 // 16384 exponentials 1024 as well.  Measured it is neither, but the chain of a
-// tile: 4096 tokens over 16384 positions, 16 heads of 128, bf16, 530 us = 907
-// TF/s (2500 cycles a tile).  P lies over S, so the next scores of a chain wait
+// tile: 4096 tokens over 16384 positions, 16 heads of 128, bf16, 535 us = 900
+// TF/s (2550 cycles a tile).  P lies over S, so the next scores of a chain wait
 // for all of its weights and then for all of P.V; of 4 warps a scheduler 0.5
 // could issue on average (2048 tokens over 8192: tensor pipe busy 43 %, issue
 // slots 36 %, exponential unit 38 %).  With a quarter of the exponentials on the
@@ -947,6 +947,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 const int chain = wg, step = split_keys ? 2 : 1;
                 const uint32_t s_at = tmem + lanes + T::COL_S + chain * 128, o_at = tmem + lanes + T::COL_O + chain * 128;
                 const int j0 = split_keys ? chain : 0;
+                bool spoiled = false;   // bf16 all the way: the row sees a value that is not finite
                 for (int j = j0; j < g.tiles; j += step) {
                     const int tile_no = tile_base + j, k0 = g.k0 + j * TKT;
                     wait_s(chain);
@@ -1002,7 +1003,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                                 const uint32_t* sw = bar.strange[tile_no & 7];
                                 if (sw[0] | sw[1] | sw[2] | sw[3])
                                     for (int i = 0; i < TKT; i++)
-                                        if ((sw[i >> 5] >> (i & 31) & 1) && k0 + i >= lo_row && k0 + i < hi_row) l = __uint_as_float(0x7fc00000u);
+                                        if ((sw[i >> 5] >> (i & 31) & 1) && k0 + i >= lo_row && k0 + i < hi_row) spoiled = true;
                             }
                         }
                         ptx::tmem_st_wait();
@@ -1021,6 +1022,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
 #pragma unroll
                         for (int b = 0; b < D; b += 32) ptx::tmem_ld32(o_at + b, reinterpret_cast<uint32_t(&)[32]>(r[b]));
                         ptx::tmem_ld_wait();
+                    }
+                    if (T::DIRECT && spoiled) {
+#pragma unroll
+                        for (int i = 0; i < NO; i++) o[i] = __uint_as_float(0x7fc00000u);
                     }
                     ptx::tc_fence_before();
                 }

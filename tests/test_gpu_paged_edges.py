@@ -515,3 +515,21 @@ def test_calls_of_two_launches_in_a_graph(paged, cache, act, hq, lens, new):
         want, wacc = settle(*(t.cpu().numpy() for t in (target, draft, x, au, su)))
         np.testing.assert_array_equal(accepted.cpu().numpy(), wacc)
         np.testing.assert_array_equal(tokens.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("cache,act", CACHES)
+@pytest.mark.parametrize("new,lens", [(1, 40), (5, 3000), (60, 300), (300, 500)])
+def test_values_do_not_enter_the_log_sum_exp(paged, cache, act, new, lens):
+    """A value that is not finite makes outputs NaN; the softmax's sum knows nothing of it."""
+    s = Setup(cache, act, 4, 2, 64, 16, [lens], [new], seed=44)
+    _, want = s.expected()
+    for pos in (lens - 1, lens - new // 2 - 1, 3):
+        pg, off = place(s, 0, pos)
+        if s.scale["v"] is None:
+            s.pages["v"][pg, off, 0, 5] = math.nan
+        else:
+            s.scale["v"][pg, off, 0] = math.nan
+    lse = torch.empty(s.q.shape[:2], device="cuda")
+    out = s.attend(paged, lse=lse)
+    assert bool(out[:, :2].isnan().any(-1).all()) and bool(out[:, 2:].isfinite().all())
+    assert float((lse.double() - want).abs().max()) < (1e-4 if act == "f32" else 2e-2)
