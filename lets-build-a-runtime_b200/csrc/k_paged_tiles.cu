@@ -813,10 +813,13 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 }
                 const bool raise = top > m + RAISE, wider = !T::DIRECT && tile_v > v_top;
                 if (!raise && !wider) return 1.0f;
+                const bool first = m == -INFINITY;   // (nothing summed yet: o = 0)
                 if (raise) m = top;
                 if (wider) v_top = 4.0f * tile_v;
                 const float to = (m == -INFINITY ? 0.0f : m) + (T::DIRECT ? 0.0f : fmaxf(log2f(v_top), -100.0f) - W_LOG2);
-                const float f = l == 0.0f ? 0.0f : exp2_fast(ref - to);   // (nothing summed yet: o = 0)
+                // (by the row's maximum: the weight sum of a thread that has half of the row's positions may
+                // be 0 where the other's is not, and its share of the output has both)
+                const float f = first ? 0.0f : exp2_fast(ref - to);
                 ref = to;
                 l *= f;
                 return f;

@@ -533,3 +533,31 @@ def test_values_do_not_enter_the_log_sum_exp(paged, cache, act, new, lens):
     out = s.attend(paged, lse=lse)
     assert bool(out[:, :2].isnan().any(-1).all()) and bool(out[:, 2:].isfinite().all())
     assert float((lse.double() - want).abs().max()) < (1e-4 if act == "f32" else 2e-2)
+
+
+@pytest.mark.parametrize("cache,act", CACHES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sink", [0, 70, 130, 200])
+def test_a_position_that_outweighs_all_others(paged, cache, act, dim, sink):
+    """One key with a score some 200 above the rest, and larger values far behind it: every weight but one
+    underflows, and the output is that position's values."""
+    s = Setup(cache, act, 32, 16, dim, 16, [1500, 900, 1200, 1400, 1100], [100, 100, 64, 80, 90], seed=46)
+    for b, n in enumerate(s.lens):
+        at = place(s, b, sink)
+        if s.scale["k"] is None:
+            s.pages["k"][at] = 8.0
+        else:
+            s.pages["k"][at] = torch.full((dim,), 100.0, device="cuda").to(CACHE[cache])
+            s.scale["k"][at] = 0.08
+        for i in range(384 // 16, -(-n // 16)):         # whole pages
+            pg = int(s.table[b, i])
+            if s.scale["v"] is None:
+                s.pages["v"][pg] *= 16
+            else:
+                s.scale["v"][pg] *= 16
+    s.q.copy_((200 * dim ** 0.5 / (8 * dim) + 0.1 * s.q.float()).to(s.q.dtype))
+    out = s.attend(paged)
+    ref, _ = s.expected()
+    assert bool(out.isfinite().all())
+    # the one weight is 1 up to fp32 rounding: the values' own form (22 bits), then the output's rounding
+    assert float((out.double() - ref).abs().max()) <= (2.0 ** -19 if act == "f32" else 2.0 ** -8) * float(ref.abs().max())
