@@ -60,7 +60,7 @@ static_assert(REG_LOAD + REG_MMA + 2 * REG_SOFT <= 512, "four warpgroups share 5
 constexpr uint64_t WAIT_NS = 2000000000ull;
 constexpr int ERR_P_LOAD = 0x501, ERR_P_MMA = 0x502, ERR_P_SOFT = 0x503, ERR_P_SMEM = 0x505;
 constexpr float RAISE = 8.0f;      // the reference moves when a score passes it by this (log2)
-constexpr float W_LOG2 = 6.0f;     // fp16 weights reach 2^8 * 2^6
+constexpr int W_LOG2 = 6;          // fp16 weights reach 2^8 * 2^6 (* 2: value scales count by their exponent)
 
 template <int CT, bool F32ACT, int D>
 struct Tile {
@@ -767,7 +767,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
             const int at_pos = s.L - s.n + my_row / p.group;
             const int lo_row = paged_lo(p, at_pos);
             const int hi_row = live ? (p.a.causal ? min(s.L, at_pos + 1) : s.L) : 0;
-            float c_row = base, m = -INFINITY, l = 0.0f, ref = 0.0f, v_top = 0.0f;   // ref: what exponents are taken against
+            // m, l: the row's maximum (as of the last move) and its weight sum in units of 2^m. Exponents are
+            // taken against ref = m + the exponent of the value scales: weights times scales are then in
+            // fp16's range, and O is in units of `unit` = 2^(ref - m), which l, with no values in it, is not.
+            float c_row = base, m = -INFINITY, l = 0.0f, ref = 0.0f, v_top = 0.0f, unit = 1.0f;
             // Scores of N positions from b on: times their scales, -inf where the row does not see them; their maximum.
             auto see = [&](auto& x, int b, int tile_no, int k0, bool masked) -> float {
                 constexpr int N = sizeof(x) / 4;
@@ -814,14 +817,18 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 const bool raise = top > m + RAISE, wider = !T::DIRECT && tile_v > v_top;
                 if (!raise && !wider) return 1.0f;
                 const bool first = m == -INFINITY;   // (nothing summed yet: o = 0)
-                if (raise) m = top;
+                if (raise) {
+                    if (!first) l *= exp2_fast(m - top);
+                    m = top;
+                }
                 if (wider) v_top = 4.0f * tile_v;
-                const float to = (m == -INFINITY ? 0.0f : m) + (T::DIRECT ? 0.0f : fmaxf(log2f(v_top), -100.0f) - W_LOG2);
+                const int shift = T::DIRECT ? 0 : max((int)(__float_as_uint(v_top) >> 23) - 127, -100) - W_LOG2;
+                const float to = (m == -INFINITY ? 0.0f : m) + (float)shift;
                 // (by the row's maximum: the weight sum of a thread that has half of the row's positions may
                 // be 0 where the other's is not, and its share of the output has both)
                 const float f = first ? 0.0f : exp2_fast(ref - to);
                 ref = to;
-                l *= f;
+                if constexpr (!T::DIRECT) unit = pow2i(shift);
                 return f;
             };
             // Scores to weights, in place; their sum.  Then times the value scales.
@@ -840,7 +847,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 }
                 float a, c2;
                 upk2(add2(s0, s1), a, c2);
-                l += a + c2;
+                l += T::DIRECT ? a + c2 : (a + c2) * unit;
                 if constexpr (!T::DIRECT) {
                     const float* vs = reinterpret_cast<const float*>(smem + T::OFF_VS) + tile_no % T::VSD * 128 + b;
 #pragma unroll
@@ -936,6 +943,8 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                     if (ok && any_live) fold(j & 1);
                 }
                 if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < NO; i++) o[i] *= unit;
                 ptx::tc_fence_before();
                 if (any_live) {   // the weight sum of both halves
                     const int t = g.tiles & 1;
@@ -1026,6 +1035,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         for (int b = 0; b < D; b += 32) ptx::tmem_ld32(o_at + b, reinterpret_cast<uint32_t(&)[32]>(r[b]));
                         ptx::tmem_ld_wait();
                     }
+                    if constexpr (!T::DIRECT) {
+#pragma unroll
+                        for (int i = 0; i < NO; i++) o[i] *= unit;
+                    }
                     if (T::DIRECT && spoiled) {
 #pragma unroll
                         for (int i = 0; i < NO; i++) o[i] = __uint_as_float(0x7fc00000u);
@@ -1035,21 +1048,18 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                 if (split_keys) {   // the other chain's share of the keys
                     float* x = reinterpret_cast<float*>(smem + T::QP * T::PLANE);   // the second Q tile's place
                     if (chain == 1) {
-                        x[row] = l == 0.0f ? -INFINITY : ref;
+                        x[row] = m;
                         x[128 + row] = l;
                     }
                     meet();
                     if (!ok) break;
                     float f0 = 1.0f, f1 = 0.0f;
-                    if (chain == 0) {
-                        const float r1 = x[row], l1 = x[128 + row];
-                        const float r0 = l == 0.0f ? -INFINITY : ref, to = fmaxf(r0, r1);
-                        if (to != -INFINITY) {
-                            f0 = l == 0.0f ? 0.0f : exp2_fast(r0 - to);
-                            f1 = l1 == 0.0f ? 0.0f : exp2_fast(r1 - to);
-                            l = l * f0 + l1 * f1;
-                            ref = to;
-                        }
+                    if (chain == 0) {   // (a sum of NaN has no maximum to go by, and goes into the result)
+                        const float m1 = x[row], l1 = x[128 + row], to = fmaxf(m, m1);
+                        f0 = l == 0.0f ? 0.0f : l == l ? exp2_fast(m - to) : l;
+                        f1 = l1 == 0.0f ? 0.0f : l1 == l1 ? exp2_fast(m1 - to) : l1;
+                        l = l * f0 + l1 * f1;
+                        m = to;
                     }
                     meet();
                     if (!ok) break;
@@ -1094,7 +1104,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
                         for (int i = 0; i < NO / 4; i++)
                             out[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
                     }
-                    if (col0 == 0) paged_store_lse(p, s, cur.h, my_row, ref, l);
+                    if (col0 == 0) paged_store_lse(p, s, cur.h, my_row, m, l);
                 } else {
                     float* part = p.part + (int64_t)(2 * blockIdx.x + (cur.i == 0)) * T::OUT;
                     const int r = my_row - g.row0;
@@ -1102,7 +1112,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tiles_kernel(const __grid_constan
 #pragma unroll
                     for (int i = 0; i < NO / 4; i++) out[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     if (col0 == 0) {
-                        part[T::R * D + r] = l == 0.0f ? -INFINITY : ref;
+                        part[T::R * D + r] = m;
                         part[T::R * D + T::R + r] = l;
                     }
                 }

@@ -536,6 +536,28 @@ def test_values_do_not_enter_the_log_sum_exp(paged, cache, act, new, lens):
 
 
 @pytest.mark.parametrize("cache,act", CACHES)
+@pytest.mark.parametrize("heads,seqs,new", [(2, 1, 1), (2, 1, 80), (16, 4, 80), (8, 3, 200)])
+@pytest.mark.parametrize("powers", [(None, 40), (None, 60), (-60, 60), (60, None), (-40, None, 40, 0)])
+def test_values_of_far_apart_sizes(paged, cache, act, heads, seqs, new, powers):
+    """Values of every 128 positions times a power of two of their own, or zero: what weighs little in the output
+    still weighs in full in the sum and the log-sum-exp."""
+    s = Setup(cache, act, heads, heads, 64, 16, [700 + 30 * b for b in range(seqs)], [new] * seqs, seed=45)
+    for b, n in enumerate(s.lens):
+        for i in range(0, n, 16):
+            f, pg = powers[i // 128 % len(powers)], int(s.table[b, i // 16])
+            f = 0.0 if f is None else 2.0 ** f
+            if s.scale["v"] is None:
+                s.pages["v"][pg] = torch.where(s.pages["v"][pg].isnan(), s.pages["v"][pg], s.pages["v"][pg] * f)
+            else:
+                s.scale["v"][pg] *= f
+    lse = torch.empty(s.q.shape[:2], device="cuda")
+    out = s.attend(paged, lse=lse)
+    ref, want = s.expected()
+    compare(s, out, act)
+    assert float((lse.double() - want).abs().max()) < (1e-4 if act == "f32" else 2e-2)
+
+
+@pytest.mark.parametrize("cache,act", CACHES)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("sink", [0, 70, 130, 200])
 def test_a_position_that_outweighs_all_others(paged, cache, act, dim, sink):
