@@ -37,8 +37,8 @@
 // Scores, maxima, weight sums and outputs are fp32.
 //
 // Measured: 64 sequences of up to 8192 positions, one token each, 8 heads of
-// 128: int8 168 us = 3.8 TB/s, bf16 262 = 4.8, fp32 625 = 4.0; two of 131072
-// in bf16 211 us = 5.0 TB/s.  8-bit caches are bound by the chain of dependent
+// 128: int8 164 us = 3.9 TB/s, bf16 262 = 4.8, fp32 625 = 4.0; two of 131072
+// in bf16 210 us = 5.1 TB/s.  8-bit caches are bound by the chain of dependent
 // instructions of three warps a scheduler (issue slots 44 % busy, DRAM 47 %;
 // the registers allow no fourth warp), and half of what is issued is the
 // copies: a look-up and an address for each 128 bytes, scales 4 bytes at a time;

@@ -31,7 +31,7 @@
 //
 // Bound: the two products of a 128 x 128 tile take 1024 cycles at D = 128, its
 // 16384 exponentials 1024 as well.  Measured it is neither, but the chain of a
-// tile: 4096 tokens over 16384 positions, 16 heads of 128, bf16, 535 us = 900
+// tile: 4096 tokens over 16384 positions, 16 heads of 128, bf16, 537 us = 897
 // TF/s (2550 cycles a tile).  P lies over S, so the next scores of a chain wait
 // for all of its weights and then for all of P.V; of 4 warps a scheduler 0.5
 // could issue on average (2048 tokens over 8192: tensor pipe busy 43 %, issue
@@ -39,9 +39,9 @@
 // FMA pipe instead it was slower (566 -> 628 us when measured), and with waits
 // that poll harder (574 - 628).  fp32 activations have two products for one, two
 // threads a row that exchange their maximum, and weights in two parts: 12 heads
-// of 64 over int8, chunks of up to 1400 tokens, 495 us = 154 TF/s of plain
+// of 64 over int8, chunks of up to 1400 tokens, 490 us = 155 TF/s of plain
 // products (chunks of 700: tensor pipe 25 %, issue slots 41 %).  128 registers a
-// thread at launch cost every instance 400 - 700 bytes of spills.
+// thread at launch cost every instance 400 - 730 bytes of spills.
 #include <cuda_fp16.h>
 
 #include <algorithm>

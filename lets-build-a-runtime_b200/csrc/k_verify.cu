@@ -23,9 +23,9 @@
 // A warp copies, the others sum: what a block has under way is then bound by
 // the ring alone, and one block of 16 + 1 warps per SM with six slots of 2 x 16
 // KB does better than several smaller ones (128 rows of 131071 entries, fp32
-// target and draft, 134 MB: 25 us = 5.3 TB/s; two blocks with 5 x 16 KB 30,
+// target and draft, 134 MB: 26 us = 5.2 TB/s; two blocks with 5 x 16 KB 30,
 // three with 3 x 16 KB 35; loads into registers without a ring 50).  One
-// sequence of 32000 entries takes 6.7 us, of which the loads that follow from
+// sequence of 32000 entries takes 7.2 us, of which the loads that follow from
 // one another (lengths, drafts, their probabilities, the row) are the most.
 #include <cuda_bf16.h>
 
